@@ -265,6 +265,132 @@ int ls_stream_run(void* decoder, const ls_stream_layer* layers, uint32_t count, 
  * word, as a real transport error does. */
 int ls_stream_inject_copy_error(void* decoder, uint32_t group, int32_t error);
 
+/* ---- the operators around the MLP of a decode step ----
+ * LeanStream leaves them to the application (its Ministral example decodes with kernels of its own:
+ * examples/ministral/python/attention_decode_kernels.py:5-97 for rotary positions and grouped-query
+ * attention, native/predictor_shared_input.cu:16-41 for the norm). Each call is one block of arguments,
+ * checked on the host and put on `stream`; it allocates nothing, never synchronizes and can be captured
+ * into a graph. Blocks are plain data and can be reused. Strides are in elements, the last dimension of
+ * every tensor is contiguous, and lengths that only the device knows (q_start, context) are read there.
+ * A block's optional `status` word (device-visible) gets LS_STATUS_RANGE for a sequence whose lengths do
+ * not fit its bounds and LS_STATUS_BAD_DESCRIPTOR for a visible key without a valid page; it is never
+ * cleared by a call. Return values: 0, EINVAL for an inconsistent block, ENOTSUP for a shape without
+ * kernels, ENOSPC for too small a workspace, or a hipError_t. */
+enum { LS_TYPE_F16 = 0, LS_TYPE_BF16 = 1, LS_TYPE_F32 = 2 };
+
+/* Attention of new tokens over a paged cache. Token i of sequence s (its n = q_start[s + 1] - q_start[s]
+ * tokens follow one another in q) stands at position p = context[s] - n + i and sees the keys j <= p, with
+ * a window only those with j > p - window or j < sinks:
+ *   out = sum_j softmax_j(scale q . k_j) v_j, 0 for a token that sees no key;
+ *   lse = log sum_j exp(scale q . k_j), -inf for such a token (optional, fp32 [tokens][q_heads]).
+ * Query head h reads KV head h / (q_heads / kv_heads). Key j of sequence s is slot j % page_size of page
+ * page_table[s * table_stride + j / page_size]; entries of pages that no token sees are not read as pages
+ * (any value). Slots that a token does not see do not change its result, whatever they hold. A sequence
+ * whose lengths are out of bounds counts as one with no keys (status RANGE); a key in a page outside
+ * [0, pages) as a key and value of zeros (status BAD_DESCRIPTOR).
+ * head_dim 64, 128 or 256; page_size a power of two; F16 or BF16 throughout; every pointer 16-byte
+ * aligned and strides multiples of 8. The workspace (ls_hip_attention_workspace bytes, zeroed once by the
+ * caller, then left alone) may be shared by calls that follow one another on one stream. */
+typedef struct ls_hip_attention {
+    const void* q;                /* [tokens][q_heads][head_dim] */
+    void* out;                    /* [tokens][q_heads][head_dim] */
+    float* lse;
+    const void* k_pages;          /* [pages][kv_heads][page_size][head_dim], in any order of strides */
+    const void* v_pages;
+    const int32_t* page_table;    /* [sequences][table_width] */
+    const int32_t* q_start;       /* [sequences + 1] */
+    const int32_t* context;       /* [sequences], new tokens included */
+    void* workspace;
+    uint32_t* status;
+    uint64_t workspace_bytes;
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    int64_t k_page_stride, k_head_stride, k_slot_stride, v_page_stride, v_head_stride, v_slot_stride;
+    int64_t table_stride;
+    uint32_t tokens, sequences, q_heads, kv_heads, head_dim, pages, page_size, table_width;
+    uint32_t max_new, max_context; /* bounds of a sequence's n and context */
+    uint32_t window, sinks;        /* window 0: none */
+    uint32_t dtype;
+    float scale;
+} ls_hip_attention;
+uint64_t ls_hip_attention_workspace(const ls_hip_attention* attention);
+int ls_hip_attention_enqueue(const ls_hip_attention* attention, void* stream);
+
+/* New tokens into a paged cache: q_out = rotated q; each token's rotated k and its v into the slot of its
+ * position (positions, q_start, context, page_table as above). Rotary pairs (i, i + rot / 2), or
+ * (2i, 2i + 1) when interleaved: a' = a cos - b sin, b' = b cos + a sin with row p of the fp32 tables,
+ * rounded once; dimensions from rot on are copied. rot 0 copies everything (cos and sin NULL). A token at a
+ * negative position, or from `positions` on with rot > 0, or without a valid page is left out (its q_out
+ * row too) and raises the status. q and q_out may be one tensor. head_dim even; F16 or BF16. */
+typedef struct ls_hip_append {
+    const void* q;                /* [tokens][q_heads][head_dim], or NULL with q_heads 0 */
+    const void* k;                /* [tokens][kv_heads][head_dim] */
+    const void* v;
+    const float* cos;             /* [positions][rot / 2] */
+    const float* sin;
+    void* q_out;
+    void* k_pages;
+    void* v_pages;
+    const int32_t* page_table;
+    const int32_t* q_start;
+    const int32_t* context;
+    uint32_t* status;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int64_t q_out_token_stride, q_out_head_stride;
+    int64_t k_page_stride, k_head_page_stride, k_slot_stride, v_page_stride, v_head_page_stride, v_slot_stride;
+    int64_t table_stride;
+    uint32_t tokens, sequences, q_heads, kv_heads, head_dim, rot, positions, pages, page_size, table_width;
+    uint32_t interleaved, dtype;
+} ls_hip_append;
+int ls_hip_append_enqueue(const ls_hip_append* append, void* stream);
+
+/* Between two blocks, row by row, in fp32 and rounded once per output:
+ *   z = post_weight ? block / rms(block) * (weight_offset + post_weight) : block
+ *   h = residual_scale * residual + gate * z          (gate absent: 1)
+ *   hidden = h; normed = h / rms(h) * (weight_offset + pre_weight)
+ * with rms(x) = sqrt(mean(x^2) + eps). gate_stride 0: one gate row for all. hidden or normed may be NULL
+ * (not both; normed needs pre_weight); hidden may be residual, and either may be block. width <= 16384,
+ * F16, BF16 or F32 throughout, any alignment of an element. */
+typedef struct ls_hip_block_norm {
+    const void* block;
+    const void* residual;
+    const void* gate;
+    const void* post_weight;
+    const void* pre_weight;
+    void* hidden;
+    void* normed;
+    int64_t block_stride, residual_stride, gate_stride, hidden_stride, normed_stride;
+    uint32_t rows, width, dtype;
+    float residual_scale, weight_offset, eps;
+} ls_hip_block_norm;
+int ls_hip_block_norm_enqueue(const ls_hip_block_norm* norm, void* stream);
+
+/* One token a row from given random numbers. With top the row's largest logit, e_i = exp((l_i - top) / T)
+ * in fp32 and w_i = e_i rounded to whole steps of 2^-32: of the tokens ranked by (logit descending, id
+ * ascending) keep the first top_k (top_k <= 0: all), of these those whose better-ranked ones weigh less
+ * than top_p of all of these, of these those with e_i >= min_p; the best one always stays. The token is
+ * the lowest kept id whose weight with the kept ids below it exceeds uniform * (kept weight). Weights are
+ * summed as whole numbers and shares are taken in steps of 2^-24, so the result does not depend on an
+ * order of summation. temperature <= 0: the best token. NaN logits count as -inf; a row without a logit
+ * above -inf gives token -1 and logprob -inf. logprob (optional) = log e_token - log(kept weight / 2^32).
+ * temperature, top_k, top_p, min_p: per row, or NULL for 1, all, 1, 0. vocab <= 2^20.
+ * The workspace: as for attention, of ls_hip_sample_workspace bytes. */
+typedef struct ls_hip_sample {
+    const void* logits;           /* [rows][vocab], F16, BF16 or F32 */
+    const float* uniform;         /* [rows] in [0, 1) */
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    int32_t* tokens;
+    float* logprob;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int64_t row_stride;
+    uint32_t rows, vocab, dtype;
+} ls_hip_sample;
+uint64_t ls_hip_sample_workspace(const ls_hip_sample* sample);
+int ls_hip_sample_enqueue(const ls_hip_sample* sample, void* stream);
+
 /* ---- synthetic workload generation on the device (counter-based splitmix64) ---- */
 int ls_synth_bytes(void* dst, uint64_t bytes, uint64_t seed, void* stream);
 int ls_synth_uniform_f16(void* dst, uint64_t count, uint64_t seed, double lo, double hi, void* stream);

@@ -13,6 +13,7 @@ p = C.c_void_p
 u32 = C.c_uint32
 u64 = C.c_uint64
 i32 = C.c_int32
+i64 = C.c_int64
 
 
 class ExecDesc(C.Structure):
@@ -75,6 +76,50 @@ class StreamLayer(C.Structure):
                 ("arrival_ns", p), ("input", p), ("output", p)]
 
 
+class Attention(C.Structure):
+    """ls_hip_attention (include/leanstream_hip.h)."""
+
+    _fields_ = [("q", p), ("out", p), ("lse", p), ("k_pages", p), ("v_pages", p), ("page_table", p), ("q_start", p),
+                ("context", p), ("workspace", p), ("status", p), ("workspace_bytes", u64),
+                ("q_token_stride", i64), ("q_head_stride", i64), ("out_token_stride", i64), ("out_head_stride", i64),
+                ("k_page_stride", i64), ("k_head_stride", i64), ("k_slot_stride", i64),
+                ("v_page_stride", i64), ("v_head_stride", i64), ("v_slot_stride", i64), ("table_stride", i64),
+                ("tokens", u32), ("sequences", u32), ("q_heads", u32), ("kv_heads", u32), ("head_dim", u32),
+                ("pages", u32), ("page_size", u32), ("table_width", u32), ("max_new", u32), ("max_context", u32),
+                ("window", u32), ("sinks", u32), ("dtype", u32), ("scale", C.c_float)]
+
+
+class Append(C.Structure):
+    """ls_hip_append (include/leanstream_hip.h)."""
+
+    _fields_ = [("q", p), ("k", p), ("v", p), ("cos", p), ("sin", p), ("q_out", p), ("k_pages", p), ("v_pages", p),
+                ("page_table", p), ("q_start", p), ("context", p), ("status", p),
+                ("q_token_stride", i64), ("q_head_stride", i64), ("k_token_stride", i64), ("k_head_stride", i64),
+                ("v_token_stride", i64), ("v_head_stride", i64), ("q_out_token_stride", i64),
+                ("q_out_head_stride", i64), ("k_page_stride", i64), ("k_head_page_stride", i64),
+                ("k_slot_stride", i64), ("v_page_stride", i64), ("v_head_page_stride", i64), ("v_slot_stride", i64),
+                ("table_stride", i64), ("tokens", u32), ("sequences", u32), ("q_heads", u32), ("kv_heads", u32),
+                ("head_dim", u32), ("rot", u32), ("positions", u32), ("pages", u32), ("page_size", u32),
+                ("table_width", u32), ("interleaved", u32), ("dtype", u32)]
+
+
+class BlockNorm(C.Structure):
+    """ls_hip_block_norm (include/leanstream_hip.h)."""
+
+    _fields_ = [("block", p), ("residual", p), ("gate", p), ("post_weight", p), ("pre_weight", p), ("hidden", p),
+                ("normed", p), ("block_stride", i64), ("residual_stride", i64), ("gate_stride", i64),
+                ("hidden_stride", i64), ("normed_stride", i64), ("rows", u32), ("width", u32), ("dtype", u32),
+                ("residual_scale", C.c_float), ("weight_offset", C.c_float), ("eps", C.c_float)]
+
+
+class Sample(C.Structure):
+    """ls_hip_sample (include/leanstream_hip.h)."""
+
+    _fields_ = [("logits", p), ("uniform", p), ("temperature", p), ("top_k", p), ("top_p", p), ("min_p", p),
+                ("tokens", p), ("logprob", p), ("workspace", p), ("workspace_bytes", u64), ("row_stride", i64),
+                ("rows", u32), ("vocab", u32), ("dtype", u32)]
+
+
 _SIGNATURES = [
     ("ls_hip_create", [], p),
     ("ls_hip_create_table", [p, u32, u32], p),
@@ -122,6 +167,12 @@ _SIGNATURES = [
     ("ls_stream_queue", [p, p], C.c_int),
     ("ls_stream_run", [p, p, u32, u32, p, p, p, i32], C.c_int),
     ("ls_stream_inject_copy_error", [p, u32, i32], C.c_int),
+    ("ls_hip_attention_workspace", [p], u64),
+    ("ls_hip_attention_enqueue", [p, p], C.c_int),
+    ("ls_hip_append_enqueue", [p, p], C.c_int),
+    ("ls_hip_block_norm_enqueue", [p, p], C.c_int),
+    ("ls_hip_sample_workspace", [p], u64),
+    ("ls_hip_sample_enqueue", [p, p], C.c_int),
     ("ls_synth_bytes", [p, u64, u64, p], C.c_int),
     ("ls_synth_uniform_f16", [p, u64, u64, C.c_double, C.c_double, p], C.c_int),
     ("ls_synth_normal_f16", [p, u64, u64, p], C.c_int),
