@@ -17,119 +17,232 @@ __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(_Float16 x) { return (float)x; }
 __device__ __forceinline__ float to_float(__bf16 x) { return (float)x; }
 
-__device__ __forceinline__ float block_sum(float x, float* scratch) {
+// Eight elements at any element's alignment, loaded and stored as 16-byte words.
+template <class T>
+struct Vec8 {
+    typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    typedef T half __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
+
+// The i-th eight of a row of `width` elements; zeros beyond its end.
+template <class T>
+__device__ __forceinline__ typename Vec8<T>::type load8(const T* row, uint32_t i, uint32_t width) {
+    typename Vec8<T>::type v = {};
+    if (8 * i + 8 <= width) v = *(const typename Vec8<T>::type*)(row + 8 * i);
+    else
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (8 * i + j < width) v[j] = row[8 * i + j];
+    return v;
+}
+template <class T>
+__device__ __forceinline__ void store8(T* row, uint32_t i, uint32_t width, const float (&x)[8]) {
+    typename Vec8<T>::type v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (T)x[j];
+    if (8 * i + 8 <= width) *(typename Vec8<T>::type*)(row + 8 * i) = v;
+    else
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (8 * i + j < width) row[8 * i + j] = v[j];
+}
+
+// Sum over the waves of a row.
+template <int Waves>
+__device__ __forceinline__ float row_sum(float x, float* scratch) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = 0.0f;
-    for (int i = 0; i < kThreads / 64; ++i) x += scratch[i];
+    if constexpr (Waves > 1) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Waves; ++i) x += scratch[i];
+    }
     return x;
 }
 
-// One workgroup a row. The row of z, then of h, stays in LDS (fp32) between the passes.
-template <class T>
+// Bound by memory: every input is read once, all of a thread's loads are under way before the first sum, and
+// the row stays in registers (fp32) from there on. Rows of up to 2048 columns take one wave (no barriers),
+// four to a workgroup; longer ones the whole workgroup. Vecs: eights of a thread.
+template <class T, int Waves, int Vecs>
 __global__ __launch_bounds__(kThreads) void block_norm_kernel(const ls_hip_block_norm a) {
-    extern __shared__ float row[];
-    __shared__ float scratch[kThreads / 64];
-    const int64_t r = blockIdx.x;
+    __shared__ float scratch[Waves];
+    constexpr uint32_t kLanes = 64 * Waves;
+    const int64_t r = Waves > 1 ? blockIdx.x : blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    if (r >= (int64_t)a.rows) return;   // a wave of its own row: no barrier follows
+    const uint32_t lane = threadIdx.x % kLanes, width = a.width;
     const T* block = (const T*)a.block + r * a.block_stride;
     const T* residual = (const T*)a.residual + r * a.residual_stride;
     const T* gate = (const T*)a.gate + r * a.gate_stride;
     const T* post = (const T*)a.post_weight;
     const T* pre = (const T*)a.pre_weight;
-    const float n = (float)a.width;
+    const float n = (float)width;
 
-    float sum = 0.0f;
-    for (uint32_t i = threadIdx.x; i < a.width; i += kThreads) {
-        const float y = to_float(block[i]);
-        row[i] = y;
-        sum += y * y;
-    }
+    typename Vec8<T>::type y[Vecs], res[Vecs], gt[Vecs] = {};
+#pragma unroll
+    for (int v = 0; v < Vecs; ++v) y[v] = load8(block, lane + v * kLanes, width);
+#pragma unroll
+    for (int v = 0; v < Vecs; ++v) res[v] = load8(residual, lane + v * kLanes, width);
+    if (gate)
+#pragma unroll
+        for (int v = 0; v < Vecs; ++v) gt[v] = load8(gate, lane + v * kLanes, width);
+
     float inv = 1.0f;
-    if (post) inv = 1.0f / sqrtf(block_sum(sum, scratch) / n + a.eps);
-    sum = 0.0f;
-    for (uint32_t i = threadIdx.x; i < a.width; i += kThreads) {
-        float z = row[i];
-        if (post) z = z * inv * (a.weight_offset + to_float(post[i]));
-        if (a.gate) z *= to_float(gate[i]);
-        const float h = a.residual_scale * to_float(residual[i]) + z;
-        row[i] = h;
-        sum += h * h;
+    if (post) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < Vecs; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += to_float(y[v][j]) * to_float(y[v][j]);
+        inv = 1.0f / sqrtf(row_sum<Waves>(sum, scratch) / n + a.eps);
     }
-    if (a.normed) inv = 1.0f / sqrtf(block_sum(sum, scratch) / n + a.eps);
-    else __syncthreads();
-    for (uint32_t i = threadIdx.x; i < a.width; i += kThreads) {
-        const float h = row[i];
-        if (a.hidden) ((T*)a.hidden)[r * a.hidden_stride + i] = (T)h;
-        if (a.normed) ((T*)a.normed)[r * a.normed_stride + i] = (T)(h * inv * (a.weight_offset + to_float(pre[i])));
+    float h[Vecs][8], sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < Vecs; ++v) {
+        typename Vec8<T>::type w = {};
+        if (post) w = load8(post, lane + v * kLanes, width);
+        const bool in = 8 * (lane + v * kLanes) < width;   // beyond the end 0 * inv may be NaN
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float z = to_float(y[v][j]);
+            if (post) z = z * inv * (a.weight_offset + to_float(w[j]));
+            if (gate) z *= to_float(gt[v][j]);
+            h[v][j] = a.residual_scale * to_float(res[v][j]) + z;
+            if (in && 8 * (lane + v * kLanes) + j < width) sum += h[v][j] * h[v][j];
+        }
+    }
+    if (a.hidden)
+#pragma unroll
+        for (int v = 0; v < Vecs; ++v) store8((T*)a.hidden + r * a.hidden_stride, lane + v * kLanes, width, h[v]);
+    if (!a.normed) return;
+    inv = 1.0f / sqrtf(row_sum<Waves>(sum, scratch) / n + a.eps);
+#pragma unroll
+    for (int v = 0; v < Vecs; ++v) {
+        const typename Vec8<T>::type w = load8(pre, lane + v * kLanes, width);
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = h[v][j] * inv * (a.weight_offset + to_float(w[j]));
+        store8((T*)a.normed + r * a.normed_stride, lane + v * kLanes, width, x);
     }
 }
 
-// The sequence that holds row t of q: the last one that starts at or before it.
+template <class T>
+void launch_norm(const ls_hip_block_norm& a, hipStream_t st) {
+    const uint32_t w = a.width, packed = (a.rows + kThreads / 64 - 1) / (kThreads / 64);
+    if (w <= 512) block_norm_kernel<T, 1, 1><<<packed, kThreads, 0, st>>>(a);
+    else if (w <= 2048) block_norm_kernel<T, 1, 4><<<packed, kThreads, 0, st>>>(a);
+    else if (w <= 4096) block_norm_kernel<T, 4, 2><<<a.rows, kThreads, 0, st>>>(a);
+    else if (w <= 8192) block_norm_kernel<T, 4, 4><<<a.rows, kThreads, 0, st>>>(a);
+    else block_norm_kernel<T, 4, 8><<<a.rows, kThreads, 0, st>>>(a);
+}
+
+// The sequence that holds row t of q: the last one that starts at or before it, 64 candidates at a time.
 __device__ __forceinline__ int find_sequence(const int32_t* q_start, uint32_t sequences, int t) {
-    int lo = 0, hi = (int)sequences;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (q_start[mid] <= t) lo = mid;
-        else hi = mid;
+    const uint32_t lane = threadIdx.x & 63;
+    int found = 0;
+    for (uint32_t s0 = 0; s0 < sequences; s0 += 64) {
+        const uint64_t at = __ballot(s0 + lane < sequences && q_start[min(s0 + lane, sequences - 1)] <= t);
+        if (!at) break;
+        found = (int)s0 + 63 - __clzll((long long)at);
     }
-    return lo;
+    return found;
 }
 
 // One workgroup a token: its q and k heads are rotated and its k and v put into the slot of its position.
-template <class T>
+// Bound by memory (and by the latency of q_start -> context -> page for few tokens). Chunks of 8 dimensions go
+// in 16-byte words where the head and the rotated part divide into them (Wide); otherwise pairs go alone.
+template <class T, bool Wide>
 __global__ __launch_bounds__(kThreads) void append_kernel(const ls_hip_append a, uint32_t page_shift) {
     const int64_t t = blockIdx.x;
     const int s = find_sequence(a.q_start, a.sequences, (int)t);
     const int first = a.q_start[s], end = a.q_start[s + 1];
     if (t < first || t >= end) return;   // no sequence's token
-    const int pos = a.context[s] - (end - (int)t);
-    if (pos < 0 || (a.rot && (uint32_t)pos >= a.positions) || (uint32_t)(pos >> page_shift) >= a.table_width) {
+    const int64_t pos = (int64_t)a.context[s] - (end - t);
+    if (pos < 0 || (a.rot && pos >= (int64_t)a.positions) || (pos >> page_shift) >= (int64_t)a.table_width) {
         if (threadIdx.x == 0 && a.status) atomicOr(a.status, (uint32_t)LS_STATUS_RANGE);
         return;
     }
     const int page = a.page_table[s * a.table_stride + (pos >> page_shift)];
-    const int slot = pos & ((1 << page_shift) - 1);
+    const int64_t slot = pos & ((1 << page_shift) - 1);
     if ((uint32_t)page >= a.pages) {
         if (threadIdx.x == 0 && a.status) atomicOr(a.status, (uint32_t)LS_STATUS_BAD_DESCRIPTOR);
         return;
     }
-    const uint32_t pairs = a.head_dim / 2, half = a.rot / 2;
-    const float* cosine = a.cos + (int64_t)pos * half;
-    const float* sine = a.sin + (int64_t)pos * half;
-    const uint32_t heads = a.q_heads + 2 * a.kv_heads;
-    for (uint32_t i = threadIdx.x; i < heads * pairs; i += kThreads) {
-        const uint32_t head = i / pairs, j = i % pairs;
-        const T* src;
-        T* dst;
-        bool turn = j < half;
+    // units of a head: rotated ones (a pair of chunks, or of dimensions), then copied ones
+    constexpr uint32_t kUnit = Wide ? 8 : 1;
+    const uint32_t half = a.rot / 2;
+    const uint32_t turned = a.interleaved && Wide ? a.rot / 8 : half / kUnit;
+    const uint32_t plain = (a.head_dim - a.rot) / kUnit;
+    const uint32_t turn_units = (a.q_heads + a.kv_heads) * turned, plain_units = (a.q_heads + a.kv_heads) * plain;
+    const uint32_t v_units = a.kv_heads * (a.head_dim / kUnit);
+    const float* cosine = a.cos + pos * half;
+    const float* sine = a.sin + pos * half;
+    auto place = [&](uint32_t head, const T*& src, T*& dst) {
         if (head < a.q_heads) {
             src = (const T*)a.q + t * a.q_token_stride + head * a.q_head_stride;
             dst = (T*)a.q_out + t * a.q_out_token_stride + head * a.q_out_head_stride;
-        } else if (head < a.q_heads + a.kv_heads) {
-            const uint32_t h = head - a.q_heads;
-            src = (const T*)a.k + t * a.k_token_stride + h * a.k_head_stride;
-            dst = (T*)a.k_pages + page * a.k_page_stride + h * a.k_head_page_stride + slot * a.k_slot_stride;
         } else {
-            const uint32_t h = head - a.q_heads - a.kv_heads;
-            src = (const T*)a.v + t * a.v_token_stride + h * a.v_head_stride;
-            dst = (T*)a.v_pages + page * a.v_page_stride + h * a.v_head_page_stride + slot * a.v_slot_stride;
-            turn = false;
+            head -= a.q_heads;
+            src = (const T*)a.k + t * a.k_token_stride + head * a.k_head_stride;
+            dst = (T*)a.k_pages + page * a.k_page_stride + head * a.k_head_page_stride + slot * a.k_slot_stride;
         }
-        // pair j: rotated (j, j + rot / 2) or (2 j, 2 j + 1); from rot on (2 j, 2 j + 1) as they are
-        const bool apart = j < half && !a.interleaved;
-        const uint32_t x = apart ? j : 2 * j, y = apart ? j + half : 2 * j + 1;
-        const T p = src[x], q = src[y];
-        if (turn) {
-            const float c = cosine[j], sn = sine[j], u = to_float(p), v = to_float(q);
-            dst[x] = (T)(u * c - v * sn);
-            dst[y] = (T)(v * c + u * sn);
+    };
+    typedef typename Vec8<T>::type vec8;
+    typedef typename Vec8<float>::half float4u;
+    for (uint32_t i = threadIdx.x; i < turn_units; i += kThreads) {
+        const uint32_t head = i / turned, u = i % turned;
+        const T* src;
+        T* dst;
+        place(head, src, dst);
+        if constexpr (!Wide) {
+            const uint32_t x = a.interleaved ? 2 * u : u, y = a.interleaved ? 2 * u + 1 : u + half;
+            const float c = cosine[u], sn = sine[u], p = to_float(src[x]), q = to_float(src[y]);
+            dst[x] = (T)(p * c - q * sn);
+            dst[y] = (T)(q * c + p * sn);
+        } else if (a.interleaved) {   // four pairs
+            const vec8 p = *(const vec8*)(src + 8 * u);
+            const float4u c = *(const float4u*)(cosine + 4 * u), sn = *(const float4u*)(sine + 4 * u);
+            vec8 r;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = to_float(p[2 * j]), y = to_float(p[2 * j + 1]);
+                r[2 * j] = (T)(x * c[j] - y * sn[j]);
+                r[2 * j + 1] = (T)(y * c[j] + x * sn[j]);
+            }
+            *(vec8*)(dst + 8 * u) = r;
+        } else {   // eight pairs
+            const vec8 p = *(const vec8*)(src + 8 * u), q = *(const vec8*)(src + half + 8 * u);
+            const float4u c0 = *(const float4u*)(cosine + 8 * u), c1 = *(const float4u*)(cosine + 8 * u + 4);
+            const float4u s0 = *(const float4u*)(sine + 8 * u), s1 = *(const float4u*)(sine + 8 * u + 4);
+            vec8 r, w;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = to_float(p[j]), y = to_float(q[j]), c = j < 4 ? c0[j % 4] : c1[j % 4],
+                            sn = j < 4 ? s0[j % 4] : s1[j % 4];
+                r[j] = (T)(x * c - y * sn);
+                w[j] = (T)(y * c + x * sn);
+            }
+            *(vec8*)(dst + 8 * u) = r;
+            *(vec8*)(dst + half + 8 * u) = w;
+        }
+    }
+    for (uint32_t i = threadIdx.x; i < plain_units + v_units; i += kThreads) {
+        const T* src;
+        T* dst;
+        uint32_t at;
+        if (i < plain_units) {
+            place(i / plain, src, dst);
+            at = a.rot + kUnit * (i % plain);
         } else {
-            dst[x] = p;
-            dst[y] = q;
+            const uint32_t each = a.head_dim / kUnit, head = (i - plain_units) / each;
+            src = (const T*)a.v + t * a.v_token_stride + head * a.v_head_stride;
+            dst = (T*)a.v_pages + page * a.v_page_stride + head * a.v_head_page_stride + slot * a.v_slot_stride;
+            at = kUnit * ((i - plain_units) % each);
         }
+        if constexpr (Wide) *(vec8*)(dst + at) = *(const vec8*)(src + at);
+        else dst[at] = src[at];
     }
 }
 
@@ -182,10 +295,9 @@ extern "C" int ls_hip_block_norm_enqueue(const ls_hip_block_norm* a, void* strea
     if (const int rc = check(*a)) return rc;
     if (!a->rows) return 0;
     const auto st = static_cast<hipStream_t>(stream);
-    const size_t lds = a->width * sizeof(float);
-    if (a->dtype == LS_TYPE_F16) block_norm_kernel<_Float16><<<a->rows, kThreads, lds, st>>>(*a);
-    else if (a->dtype == LS_TYPE_BF16) block_norm_kernel<__bf16><<<a->rows, kThreads, lds, st>>>(*a);
-    else block_norm_kernel<float><<<a->rows, kThreads, lds, st>>>(*a);
+    if (a->dtype == LS_TYPE_F16) launch_norm<_Float16>(*a, st);
+    else if (a->dtype == LS_TYPE_BF16) launch_norm<__bf16>(*a, st);
+    else launch_norm<float>(*a, st);
     return finish();
 }
 
@@ -196,7 +308,9 @@ extern "C" int ls_hip_append_enqueue(const ls_hip_append* a, void* stream) {
     if (!a->tokens) return 0;
     const auto st = static_cast<hipStream_t>(stream);
     const uint32_t shift = __builtin_ctz(a->page_size);
-    if (a->dtype == LS_TYPE_F16) append_kernel<_Float16><<<a->tokens, kThreads, 0, st>>>(*a, shift);
-    else append_kernel<__bf16><<<a->tokens, kThreads, 0, st>>>(*a, shift);
+    const bool wide = a->head_dim % 8 == 0 && a->rot % (a->interleaved ? 8 : 16) == 0;
+    const auto kernel = a->dtype == LS_TYPE_F16 ? wide ? append_kernel<_Float16, true> : append_kernel<_Float16, false>
+                                                : wide ? append_kernel<__bf16, true> : append_kernel<__bf16, false>;
+    kernel<<<a->tokens, kThreads, 0, st>>>(*a, shift);
     return finish();
 }
