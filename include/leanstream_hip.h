@@ -364,14 +364,15 @@ typedef struct ls_hip_block_norm {
 } ls_hip_block_norm;
 int ls_hip_block_norm_enqueue(const ls_hip_block_norm* norm, void* stream);
 
-/* One token a row from given random numbers. With top the row's largest logit, e_i = exp((l_i - top) / T)
- * in fp32 and w_i = e_i rounded to whole steps of 2^-32: of the tokens ranked by (logit descending, id
- * ascending) keep the first top_k (top_k <= 0: all), of these those whose better-ranked ones weigh less
- * than top_p of all of these, of these those with e_i >= min_p; the best one always stays. The token is
- * the lowest kept id whose weight with the kept ids below it exceeds uniform * (kept weight). Weights are
- * summed as whole numbers and shares are taken in steps of 2^-24, so the result does not depend on an
- * order of summation. temperature <= 0: the best token. NaN logits count as -inf; a row without a logit
- * above -inf gives token -1 and logprob -inf. logprob (optional) = log e_token - log(kept weight / 2^32).
+/* One token a row from given random numbers. With top the row's largest logit and e_i = exp((l_i - top) / T)
+ * the tokens are ranked by (logit descending, id ascending); of them keep the first top_k (top_k <= 0: all), of
+ * these those whose better-ranked ones weigh less than top_p of all of these, of these those with e_i >= min_p;
+ * the best one always stays. The token is the lowest kept id whose weight with the kept ids below it exceeds
+ * uniform * (kept weight). Exponentials are fp32; with a filter they are weighed in whole steps of 2^-32 (less
+ * than half a step: never drawn) and top_p and uniform in steps of 2^-24, without one summed in 64-bit floats in
+ * a fixed order: equal inputs give equal results. temperature <= 0 (or NaN): the best token. NaN logits count as
+ * -inf; a row without a logit above -inf gives token -1 and logprob -inf. logprob (optional): the logarithm of
+ * e_token over the kept weight.
  * temperature, top_k, top_p, min_p: per row, or NULL for 1, all, 1, 0. vocab <= 2^20.
  * The workspace: as for attention, of ls_hip_sample_workspace bytes. */
 typedef struct ls_hip_sample {

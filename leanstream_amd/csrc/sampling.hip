@@ -1,22 +1,43 @@
 // One token a row from given random numbers: ls_hip_sample_enqueue.
 //
-// e_i = exp((l_i - top) / T), w_i = round(2^32 e_i). Ranked by (logit descending, id ascending) the kept
-// tokens are a prefix: everything above a cut logit, and of the tokens equal to it the first few by id. The
-// cut of top-k, and then that of top-p among the top k, are found by radix selection over the logits' 32-bit
-// order: 8 bits a pass, with the count and the weight of every digit. Weights are whole numbers, so sums are
-// exact and no order of atomics changes a result. Tokens of weight 0 can neither be drawn nor move a share,
-// and are left out throughout.
+// e_i = exp((l_i - top) / T), w_i = e_i in whole steps of 2^-32. Ranked by (logit descending, id ascending) the
+// kept tokens are a prefix of the ranking: everything above a cut logit, and of the tokens equal to it the
+// first few by id. Weights of a set are summed as whole numbers, so no order of atomics changes a result.
+//
+// One pass over the logits: a workgroup takes a chunk of a row and leaves its best token, the sum of its
+// exponentials and, in order of id, its candidates: as many of its largest logits as the record holds. The
+// workgroup that finishes a row last finds the cuts of top-k and of top-p among the candidates by radix
+// selection (8 bits of the logits' 32-bit order at a time, with the count and the weight of every digit).
+// Whatever lies above the largest logit that is no candidate (`outside`) is known completely. Where a cut falls
+// below:
+//  - top-p alone: the chunks also left histograms of count and weight over bins of T / 16. They name the bin of
+//    the cut, whose tokens are picked from the row (one pass of comparisons) and selected among; the chunks'
+//    weights above the cut point to the chunk that holds the token, and only that is read again;
+//  - otherwise (top-k beyond the candidates, a bin of more tokens than there is room for) the workgroup selects
+//    over the whole row.
+// Without filters the chunks' sums point to the chunk that holds the token.
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cerrno>
 #include "leanstream_hip.h"
+
+// Arrays that a closure reaches stay in registers only where it is inlined.
+#define LS_INLINE __attribute__((always_inline))
 
 namespace lsamd {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr float kUnit = 4294967296.0f;   // weight of the best token
-constexpr uint32_t kMaxVocab = 1u << 20; // sums stay below 2^52
+constexpr uint32_t kMaxVocab = 1u << 20;   // sums stay below 2^52
+constexpr uint32_t kMaxChunks = 128;       // of a row
+constexpr uint32_t kCandidates = 4096;     // of a row, 8 a thread
+constexpr uint32_t kChunkCandidates = 256; // of a chunk, at most
+constexpr uint32_t kRowBlock = 256;        // rows of a launch
+constexpr int kBins = 512;                 // steps of T / 16 down from a chunk's best logit: weights to e^-32
+constexpr int kCountShift = 46;            // a bin: count << 46 | weight (at most 2^13 tokens of up to 2^32)
+constexpr uint64_t kCounterBytes = kRowBlock * sizeof(uint32_t);
+constexpr uint32_t kAll = 0xffffffffu;
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(_Float16 x) { return (float)x; }
@@ -28,6 +49,9 @@ __device__ __forceinline__ uint32_t order_of(float l) {
     const uint32_t u = __float_as_uint(l + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float logit_of(uint32_t order) {
+    return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
 
 // floor (or ceil) of total * fraction, the fraction in steps of 2^-24 (total < 2^52)
 __device__ __forceinline__ uint64_t share(uint64_t total, float fraction, bool up) {
@@ -35,14 +59,32 @@ __device__ __forceinline__ uint64_t share(uint64_t total, float fraction, bool u
     return m * (total >> 24) + ((m * (total & 0xffffff) + (up ? 0xffffff : 0)) >> 24);
 }
 
-struct Row {
-    float top, temperature;
-    __device__ __forceinline__ float log_e(float l) const {
-        return l == top ? 0.0f : (l - top) / temperature;   // equal: also where both are infinite
+// Exponentials of a row. log2(e) / T is held in two floats, and its product with the distance is split into
+// whole and fraction before it is rounded: the error of e stays near one unit in its last place.
+struct Scale {
+    float hi, lo, bins;
+    __device__ __forceinline__ explicit Scale(float temperature) {
+        const double c = 1.4426950408889634 / (double)temperature;
+        hi = (float)c;
+        lo = hi < INFINITY ? (float)(c - (double)hi) : 0.0f;
+        bins = fminf(16.0f / temperature, 3e38f);
     }
-    __device__ __forceinline__ float e(float l) const { return expf(log_e(l)); }
+    // bin on the scale of all logits of a row, rising with the logit
+    __device__ __forceinline__ int bin(float l) const { return (int)fminf(fmaxf(floorf(l * bins), -1e9f), 1e9f); }
+    // exp((l - top) / T) 2^up for l <= top; 0 for -inf
+    __device__ __forceinline__ float e(float l, float top, int up = 0) const {
+        const float t = l - top;
+        const float whole = fmaxf(rintf(t * hi), -200.0f);
+        const float part = fmaf(t, hi, -whole) + t * lo;
+        const float x = fmaxf(ldexpf(__builtin_amdgcn_exp2f(part), (int)whole + up), 0.0f);
+        // equal also where both are infinite; NaN (-inf at an infinite temperature, an infinite scale) became 0
+        return l == top ? ldexpf(1.0f, up) : x;
+    }
+    // weight in steps of 2^-32; the best token's 2^32 is held as 2^32 - 1
+    __device__ __forceinline__ uint32_t weight(float l, float top) const {
+        return (uint32_t)fminf(rintf(e(l, top, 32)), 4294967040.0f) | (l == top ? 255u : 0u);
+    }
 };
-__device__ __forceinline__ uint64_t weight(float e) { return e == e ? (uint64_t)rintf(e * kUnit) : 0; }
 
 // A prefix of the ranking: every order above `order`, and the first `ties` ids of those equal to it.
 struct Cut {
@@ -52,60 +94,106 @@ struct Cut {
 struct Shared {
     uint64_t weights[256];
     uint32_t counts[256];
-    uint64_t wave_weight[kWaves];
-    uint32_t wave_count[kWaves];
+    uint64_t wave64[kWaves];
+    double wave_sum[kWaves];
+    uint32_t wave32[kWaves];
+    float wave_float[kWaves];
     uint64_t before_weight;
-    uint32_t before_count, digit;
+    uint32_t before_count, digit, turn, token;
+    // of the row's chunks
+    double sums[kMaxChunks];
+    uint64_t list[kMaxChunks];
+    float tops[kMaxChunks];
+    uint32_t held[kMaxChunks];
+    uint64_t bins[kBins];
 };
 
-// The shortest prefix within `limit` whose count reaches need_count or whose weight reaches need_weight; all
-// of `limit` if none does. kept_weight: the weight of that prefix.
-template <class T>
-__device__ Cut select(const T* logits, uint32_t vocab, const Row& row, Cut limit, uint32_t need_count,
-                      uint64_t need_weight, Shared& sh, uint64_t* kept_weight) {
-    uint32_t prefix = 0, before_count = 0;
+__device__ __forceinline__ uint64_t wave_max(uint64_t x) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) x = max(x, (uint64_t)__shfl_xor((unsigned long long)x, d));
+    return x;
+}
+template <class V>
+__device__ __forceinline__ V wave_upto(V x) {   // inclusive sums
+    const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const V y = __shfl_up(x, d);
+        if (lane >= (uint32_t)d) x += y;
+    }
+    return x;
+}
+// Exclusive sum over the threads, and the total. The scratch array is free again after the next barrier.
+template <class V>
+__device__ __forceinline__ V block_before(V x, V* scratch, V* total) {
+    const V upto = wave_upto(x);
+    if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = upto;
+    __syncthreads();
+    V before = 0, sum = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        if (i == (int)(threadIdx.x >> 6)) before = sum;
+        sum += scratch[i];
+    }
+    *total = sum;
+    return before + upto - x;
+}
+
+// The shortest prefix within `limit` whose count reaches need_count or whose weight reaches need_weight, of the
+// tokens that each(f) hands to f(order, weight); all of `limit` if none does. kept: the weight of that prefix.
+template <class Each>
+__device__ __forceinline__ Cut select(const Each& each, Cut limit, uint32_t need_count, uint64_t need_weight, Shared& sh, uint64_t* kept) {
+    uint32_t prefix = 0;
     uint64_t before_weight = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
         for (int i = threadIdx.x; i < 256; i += kThreads) sh.weights[i] = 0, sh.counts[i] = 0;
-        if (threadIdx.x == 0) sh.digit = 256;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < vocab; i += kThreads) {
-            const float l = to_float(logits[i]);
-            const uint32_t o = order_of(l);
-            if (o < limit.order || (shift < 24 && (o >> shift >> 8) != (prefix >> shift >> 8))) continue;
-            const uint64_t w = weight(row.e(l));
-            if (!w) continue;
-            atomicAdd(&sh.counts[o >> shift & 255], 1u);
-            atomicAdd((unsigned long long*)&sh.weights[o >> shift & 255], (unsigned long long)w);
-        }
+        each([&](uint32_t order, uint32_t weight) LS_INLINE {
+            if (!weight || order < limit.order || (shift < 24 && (order >> shift >> 8) != (prefix >> shift >> 8))) return;
+            atomicAdd(&sh.counts[order >> shift & 255], 1u);
+            atomicAdd((unsigned long long*)&sh.weights[order >> shift & 255], (unsigned long long)weight);
+        });
         __syncthreads();
-        // the first digit from above at which one of the sums is reached (at the last level a digit is one
-        // logit, and of the limit's own logit only its ties count)
-        if (threadIdx.x == 0) {
-            uint32_t c = before_count;
-            uint64_t s = before_weight;
-            for (int d = 255; d >= 0; --d) {
-                uint32_t n = sh.counts[d];
-                uint64_t w = sh.weights[d];
-                if (!n) continue;
-                if (shift == 0 && (prefix | (uint32_t)d) == limit.order && n > limit.ties) w = w / n * limit.ties, n = limit.ties;
-                if (c + n >= need_count || s + w >= need_weight) {
-                    sh.digit = d;
-                    break;
-                }
-                c += n;
-                s += w;
+        // The first digit from above at which one of the sums is reached: a lane takes four digits. At the last
+        // level a digit is one logit, and of the limit's own logit only its ties count.
+        if (threadIdx.x < 64) {
+            const uint32_t lane = threadIdx.x;
+            uint32_t n[4], c = 0;
+            uint64_t w[4], s = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t d = 255 - 4 * lane - i;
+                n[i] = sh.counts[d];
+                w[i] = sh.weights[d];
+                if (shift == 0 && (prefix | d) == limit.order && n[i] > limit.ties) w[i] = w[i] / n[i] * limit.ties, n[i] = limit.ties;
+                c += n[i];
+                s += w[i];
             }
-            sh.before_count = c;
-            sh.before_weight = s;
+            uint32_t c_before = wave_upto(c) - c;
+            uint64_t s_before = wave_upto((unsigned long long)s) - s;
+            const uint64_t reached = __ballot(c_before + c >= need_count || s_before + s >= need_weight);
+            const uint32_t at = reached ? (uint32_t)__ffsll((unsigned long long)reached) - 1 : 63u;
+            if (lane == at) {
+                uint32_t digit = 256;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (digit != 256) continue;
+                    if (reached && n[i] && (c_before + n[i] >= need_count || s_before + w[i] >= need_weight)) digit = 255 - 4 * lane - i;
+                    else c_before += n[i], s_before += w[i];
+                }
+                sh.digit = digit;
+                sh.before_count = c_before;
+                sh.before_weight = s_before;
+            }
         }
         __syncthreads();
-        before_count = sh.before_count;
-        before_weight = sh.before_weight;
         const uint32_t digit = sh.digit;
+        need_count -= need_count == kAll ? 0 : sh.before_count;
+        need_weight -= need_weight == ~0ull ? 0 : sh.before_weight;
+        before_weight += sh.before_weight;
         if (digit == 256) {   // not reached: all of the limit
-            __syncthreads();
-            *kept_weight = before_weight;
+            *kept = before_weight;
             return limit;
         }
         prefix |= digit << shift;
@@ -114,125 +202,545 @@ __device__ Cut select(const T* logits, uint32_t vocab, const Row& row, Cut limit
             const uint64_t one = sh.weights[digit] / n;
             if (prefix == limit.order) n = min(n, limit.ties);
             // ties needed for the count and for the weight, whichever is reached first
-            uint64_t ties = min((uint64_t)n, (uint64_t)(need_count - before_count));
-            ties = min(ties, (need_weight - before_weight - 1) / one + 1);
-            __syncthreads();
-            *kept_weight = before_weight + ties * one;
+            const uint64_t ties = min(min((uint64_t)n, (uint64_t)need_count), (need_weight - 1) / one + 1);
+            *kept = before_weight + ties * one;
             return Cut{prefix, (uint32_t)ties};
         }
-        __syncthreads();
     }
     return limit;
 }
 
+// What a chunk leaves for its row; the candidates (order << 32 | id) follow in order of id, then the bins.
+struct Record {
+    uint64_t best;        // order << 32 | ~id
+    double sum;           // of exp((l - top) / T), top the chunk's
+    float outside;        // the largest logit that is no candidate, -inf: none
+    uint32_t count;
+};
+
+__device__ __forceinline__ void put(uint64_t* p, uint64_t v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t get(const uint64_t* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 template <class T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a) {
-    __shared__ Shared sh;
-    __shared__ uint64_t best[kWaves];
-    const uint32_t r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const T* logits = (const T*)a.logits + (int64_t)r * a.row_stride;
+struct Vec8 {
+    typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
 
-    // the best token: highest order, lowest id
-    uint64_t mine = 0;
-    for (uint32_t i = threadIdx.x; i < a.vocab; i += kThreads)
-        mine = max(mine, (uint64_t)order_of(to_float(logits[i])) << 32 | (0xffffffffu - i));
-#pragma unroll
-    for (int d = 32; d; d >>= 1) mine = max(mine, (uint64_t)__shfl_xor((unsigned long long)mine, d));
-    if (lane == 0) best[wave] = mine;
-    __syncthreads();
-    for (int i = 0; i < kWaves; ++i) mine = max(mine, best[i]);
-    const uint32_t best_id = 0xffffffffu - (uint32_t)mine;
-    Row row{to_float(logits[best_id]), a.temperature ? a.temperature[r] : 1.0f};
-    if (!(row.top > -INFINITY)) {
-        if (threadIdx.x == 0) {
-            a.tokens[r] = -1;
-            if (a.logprob) a.logprob[r] = -INFINITY;
-        }
-        return;
-    }
-    if (!(row.temperature > 0.0f)) {
-        if (threadIdx.x == 0) {
-            a.tokens[r] = (int32_t)best_id;
-            if (a.logprob) a.logprob[r] = 0.0f;
-        }
-        return;
-    }
+struct RowArgs {
+    uint32_t chunks, room, words;   // of a row; candidates of a chunk; 8-byte words of a chunk's record
+};
 
-    const int32_t top_k = a.top_k ? a.top_k[r] : 0;
-    const float top_p = a.top_p ? a.top_p[r] : 1.0f, min_p = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
-    Cut cut{0, 0xffffffffu};
-    uint64_t total;
-    cut = select(logits, a.vocab, row, cut, top_k > 0 ? (uint32_t)top_k : 0xffffffffu, ~0ull, sh, &total);
-    if (top_p < 1.0f) {
-        const uint64_t limit = share(total, top_p, true);
-        cut = select(logits, a.vocab, row, cut, 0xffffffffu, limit ? limit : 1, sh, &total);
-    }
-
-    // Kept weight of each wave's stretch of the vocabulary: what lies above the cut, and its ties in order.
-    const uint32_t stretch = ((a.vocab + kWaves - 1) / kWaves + 63) / 64 * 64;
-    const uint32_t begin = min(wave * stretch, a.vocab), end = min(begin + stretch, a.vocab);
-    uint64_t above = 0, tie_weight = 0;
-    uint32_t ties = 0;
+// The token of the row whose kept tokens, in order of id, are those above the cut and its first ties, with
+// e >= min_p: over all of the row's logits.
+template <class T>
+__device__ __forceinline__ void draw_from_row(const T* logits, uint32_t vocab, float top, const Scale& scale, Cut cut, float min_p,
+                              float uniform, Shared& sh, uint32_t* token, uint64_t* total) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t stretch = ((vocab + kWaves - 1) / kWaves + 63) / 64 * 64;
+    const uint32_t begin = min(wave * stretch, vocab), end = min(begin + stretch, vocab);
+    uint64_t above = 0;
+    uint32_t ties = 0, tie_weight = 0;
     for (uint32_t i = begin + lane; i < end; i += 64) {
         const float l = to_float(logits[i]);
         const uint32_t o = order_of(l);
-        const float e = row.e(l);
-        if (o < cut.order || !(e >= min_p)) continue;
-        if (o == cut.order) ++ties, tie_weight = weight(e);
-        else above += weight(e);
+        if (o < cut.order || !(scale.e(l, top) >= min_p)) continue;
+        if (o == cut.order) ++ties, tie_weight = scale.weight(l, top);
+        else above += scale.weight(l, top);
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        above += __shfl_xor((unsigned long long)above, d);
-        ties += __shfl_xor(ties, d);
-        tie_weight = max(tie_weight, (uint64_t)__shfl_xor((unsigned long long)tie_weight, d));
-    }
-    if (lane == 0) sh.wave_count[wave] = ties;
+    ties = __shfl(wave_upto(ties), 63);
+    tie_weight = (uint32_t)wave_max(tie_weight);
+    above = __shfl(wave_upto((unsigned long long)above), 63);
+    __syncthreads();
+    if (lane == 0) sh.wave32[wave] = ties;
     __syncthreads();
     uint32_t ties_left = cut.ties;
-    for (uint32_t i = 0; i < wave; ++i) ties_left -= min(ties_left, sh.wave_count[i]);
-    if (lane == 0) sh.wave_weight[wave] = above + min(ties, ties_left) * tie_weight;
+    for (uint32_t i = 0; i < wave; ++i) ties_left -= min(ties_left, sh.wave32[i]);
+    if (lane == 0) sh.wave64[wave] = above + (uint64_t)min(ties, ties_left) * tie_weight;
     __syncthreads();
     uint64_t sum = 0, before = 0;
     for (uint32_t i = 0; i < kWaves; ++i) {
         if (i == wave) before = sum;
-        sum += sh.wave_weight[i];
+        sum += sh.wave64[i];
     }
-    const uint64_t target = min(share(sum, a.uniform[r], false), sum - 1);
-    if (target < before || target >= before + sh.wave_weight[wave]) return;
-    // this wave's stretch holds the token
-    uint64_t seen = before;
-    for (uint32_t i0 = begin; i0 < end; i0 += 64) {
-        const uint32_t i = i0 + lane;
-        float e = 0.0f;
-        bool keep = false, tie = false;
-        if (i < end) {
-            const float l = to_float(logits[i]);
-            const uint32_t o = order_of(l);
-            e = row.e(l);
-            tie = o == cut.order && e >= min_p;
-            keep = o > cut.order && e >= min_p;
-        }
-        const uint64_t tie_lanes = __ballot(tie);
-        if (tie && (uint32_t)__popcll(tie_lanes & ((1ull << lane) - 1)) < ties_left) keep = true;
-        ties_left -= min(ties_left, (uint32_t)__popcll(tie_lanes));
-        const uint64_t w = keep ? weight(e) : 0;
-        uint64_t upto = w;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint64_t x = __shfl_up((unsigned long long)upto, d);
-            if (lane >= (uint32_t)d) upto += x;
-        }
-        const uint64_t found = __ballot(seen + upto > target);
-        if (found) {
-            if (lane == (uint32_t)__ffsll((unsigned long long)found) - 1) {
-                a.tokens[r] = (int32_t)i;
-                // from the exponent itself: a small weight's rounding does not show in its logarithm
-                if (a.logprob) a.logprob[r] = row.log_e(to_float(logits[i])) - logf((float)sum / kUnit);
+    const uint64_t target = min(share(sum, uniform, false), sum - 1);
+    if (target >= before && target < before + sh.wave64[wave]) {   // this wave's stretch holds the token
+        for (uint32_t i0 = begin; i0 < end; i0 += 64) {
+            const uint32_t i = i0 + lane;
+            uint32_t w = 0;
+            bool tie = false;
+            if (i < end) {
+                const float l = to_float(logits[i]);
+                const uint32_t o = order_of(l);
+                const bool in = o >= cut.order && scale.e(l, top) >= min_p;
+                tie = in && o == cut.order;
+                if (in) w = scale.weight(l, top);
             }
-            return;
+            const uint64_t tie_lanes = __ballot(tie);
+            if (tie && (uint32_t)__popcll(tie_lanes & ((1ull << lane) - 1)) >= ties_left) w = 0;
+            ties_left -= min(ties_left, (uint32_t)__popcll(tie_lanes));
+            const uint64_t upto = wave_upto((unsigned long long)w);
+            const uint64_t found = __ballot(before + upto > target);
+            if (found) {
+                if (lane == 0) sh.token = i0 + (uint32_t)__ffsll((unsigned long long)found) - 1;
+                break;
+            }
+            before += __shfl((unsigned long long)upto, 63);
         }
-        seen += __shfl((unsigned long long)upto, 63);
+    }
+    __syncthreads();
+    *token = sh.token;
+    *total = sum;
+}
+
+// The token of a chunk at which the running weight of its kept tokens (units of the row's best one) passes
+// `rest`; ties_before: tokens equal to the cut in earlier chunks.
+template <class T, uint32_t Chunk>
+__device__ __forceinline__ uint32_t draw_from_chunk(const T* logits, uint32_t vocab, uint32_t chunk, float top, const Scale& scale, Cut cut,
+                                    uint32_t ties_before, double rest, Shared& sh) {
+    constexpr uint32_t kEach = Chunk / kThreads;
+    const uint32_t from = chunk * Chunk, to = min(from + Chunk, vocab);
+    float x[kEach];
+    uint32_t o[kEach], ties = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
+        const uint32_t i = from + threadIdx.x * kEach + j;
+        const float v = i < to ? to_float(logits[i]) : -INFINITY;
+        o[j] = order_of(v);
+        x[j] = v > -INFINITY && o[j] >= cut.order ? scale.e(v, top) : 0.0f;
+        ties += o[j] == cut.order;
+    }
+    uint32_t chunk_ties;
+    uint32_t tie = ties_before + block_before(ties, sh.wave32, &chunk_ties);
+    double thread_sum = 0.0;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
+        if (o[j] == cut.order && tie++ >= cut.ties) x[j] = 0.0f;
+        thread_sum += x[j];
+    }
+    double chunk_sum;
+    double before = block_before(thread_sum, sh.wave_sum, &chunk_sum);
+    // `rest` and these sums are rounded apart: the last token with weight takes what is left
+    if (threadIdx.x == 0) sh.token = kAll, sh.digit = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
+        const uint32_t i = from + threadIdx.x * kEach + j;
+        before += x[j];
+        if (x[j] > 0.0f) {
+            if (before > rest) atomicMin(&sh.token, i);
+            atomicMax(&sh.digit, i);
+        }
+    }
+    __syncthreads();
+    return min(sh.token, sh.digit);
+}
+
+template <class T, int Vecs>
+__global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a, const RowArgs rows) {
+    constexpr uint32_t kChunk = 8 * Vecs * kThreads;
+    __shared__ Shared sh;
+    __shared__ __align__(16) uint8_t marks[kChunk / 8];
+    const uint32_t r = blockIdx.y, c = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const T* logits = (const T*)a.logits + (int64_t)r * a.row_stride;
+    const uint32_t begin = c * kChunk, size = min(a.vocab - begin, kChunk);
+    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+    const bool greedy = !(temperature > 0.0f);
+    const Scale scale(greedy ? 1.0f : temperature);
+    const int32_t top_k = a.top_k ? a.top_k[r] : 0;
+    const float top_p = a.top_p ? a.top_p[r] : 1.0f, min_p = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
+    const bool by_count = top_k > 0 && (uint32_t)top_k < a.vocab, by_weight = top_p < 1.0f;
+    const bool binned = by_weight && !by_count;   // may need the histograms
+
+    // ---- the chunk: element 8 (v kThreads + thread) + j
+    float l[Vecs][8];
+    uint64_t best = 0;
+#pragma unroll
+    for (int v = 0; v < Vecs; ++v) {
+        const uint32_t i = 8 * (v * kThreads + threadIdx.x);
+        if (i + 8 <= size) {
+            const typename Vec8<T>::type x = *(const typename Vec8<T>::type*)(logits + begin + i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) l[v][j] = to_float(x[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) l[v][j] = i + j < size ? to_float(logits[begin + i + j]) : -INFINITY;
+        }
+    }
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
+#pragma unroll
+    for (int v = 0; v < Vecs; ++v)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t id = begin + 8 * (v * kThreads + threadIdx.x) + j;
+            best = max(best, (uint64_t)order_of(l[v][j]) << 32 | (uint32_t)~id);
+        }
+    best = wave_max(best);
+    if (lane == 0) sh.wave64[wave] = best;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) best = max(best, sh.wave64[i]);
+    const float chunk_top = logit_of((uint32_t)(best >> 32));
+
+    uint64_t* record = (uint64_t*)((char*)a.workspace + kCounterBytes) +
+                       ((uint64_t)r * rows.chunks + c) * rows.words;
+    double sum = 0.0;
+    const int top_bin = scale.bin(chunk_top);
+    if (!greedy) {
+        float mine = 0.0f;
+#pragma unroll
+        for (int v = 0; v < Vecs; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = l[v][j];
+                if (!(x > -INFINITY)) continue;
+                mine += scale.e(x, chunk_top);
+                const int down = top_bin - scale.bin(x);
+                if (down < kBins)
+                    atomicAdd((unsigned long long*)&sh.bins[down], 1ull << kCountShift | scale.weight(x, chunk_top));
+            }
+        sum = mine;
+#pragma unroll
+        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+        if (lane == 0) sh.wave_sum[wave] = sum;
+        __syncthreads();
+        sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) sum += sh.wave_sum[i];
+        // bins that fit into the record, as many as possible
+        if (wave == 0) {
+            uint32_t n = 0, fit = 0;
+#pragma unroll
+            for (int i = 0; i < kBins / 64; ++i) n += (uint32_t)(sh.bins[kBins / 64 * lane + i] >> kCountShift);
+            uint32_t upto = wave_upto(n) - n;
+#pragma unroll
+            for (int i = 0; i < kBins / 64; ++i) fit += (upto += (uint32_t)(sh.bins[kBins / 64 * lane + i] >> kCountShift)) <= rows.room;
+            fit = __shfl(wave_upto(fit), 63);
+            if (lane == 0) sh.digit = fit;
+        }
+        __syncthreads();
+        const int bins = (int)sh.digit;
+        if (binned)
+            for (int i = threadIdx.x; i < kBins; i += kThreads) put(record + sizeof(Record) / 8 + rows.room + i, sh.bins[i]);
+        float outside = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < Vecs; ++v) {
+            uint32_t mark = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = l[v][j];
+                if (!(x > -INFINITY)) continue;
+                if (top_bin - scale.bin(x) < bins) mark |= 1u << j;
+                else outside = fmaxf(outside, x);
+            }
+            marks[v * kThreads + threadIdx.x] = (uint8_t)mark;
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) outside = fmaxf(outside, __shfl_xor(outside, d));
+        if (lane == 0) sh.wave_float[wave] = outside;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) outside = fmaxf(outside, sh.wave_float[i]);
+        // candidates in order of id: a thread takes 32 elements' marks
+        uint32_t word = threadIdx.x < kChunk / 32 ? ((const uint32_t*)marks)[threadIdx.x] : 0u, total;
+        uint32_t at = block_before((uint32_t)__popc(word), sh.wave32, &total);
+        while (word) {
+            const uint32_t id = begin + 32 * threadIdx.x + __ffs(word) - 1;
+            word &= word - 1;
+            put(record + sizeof(Record) / 8 + at++, (uint64_t)order_of(to_float(logits[id])) << 32 | id);
+        }
+        if (threadIdx.x == 0) {
+            put(record + 1, __builtin_bit_cast(uint64_t, sum));
+            put(record + 2, (uint64_t)total << 32 | __float_as_uint(outside));
+        }
+    }
+    if (threadIdx.x == 0) put(record, best);
+
+    // ---- the row, by its last chunk. Every store of the workgroup has been acknowledged before its turn is taken.
+    if (rows.chunks > 1) {
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_s_waitcnt(0);
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t* counter = (uint32_t*)a.workspace + r;
+            sh.turn = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (sh.turn == rows.chunks - 1)   // ready for the next call
+                __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (sh.turn != rows.chunks - 1) return;
+    } else {
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+    }
+    const uint32_t words = rows.words;
+    record = (uint64_t*)((char*)a.workspace + kCounterBytes) + (uint64_t)r * rows.chunks * words;
+
+    // threads 0 .. chunks - 1 hold a record each; every thread takes some of the slots for candidates
+    const bool mine = threadIdx.x < rows.chunks;
+    best = mine ? get(record + threadIdx.x * words) : 0;
+    uint64_t tail = mine && !greedy ? get(record + threadIdx.x * words + 2) : (uint64_t)__float_as_uint(-INFINITY);
+    sum = mine && !greedy ? __builtin_bit_cast(double, get(record + threadIdx.x * words + 1)) : 0.0;
+    const uint64_t own = best;
+    best = wave_max(best);
+    __syncthreads();
+    if (lane == 0) sh.wave64[wave] = best;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) best = max(best, sh.wave64[i]);
+    const uint32_t best_id = ~(uint32_t)best;
+    const float top = logit_of((uint32_t)(best >> 32));
+    if (greedy || !(top > -INFINITY)) {
+        if (threadIdx.x == 0) {
+            const bool none = !(top > -INFINITY);
+            a.tokens[r] = none ? -1 : (int32_t)best_id;
+            if (a.logprob) a.logprob[r] = none ? -INFINITY : 0.0f;
+        }
+        return;
+    }
+    float outside = __uint_as_float((uint32_t)tail);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) outside = fmaxf(outside, __shfl_xor(outside, d));
+    if (lane == 0) sh.wave_float[wave] = outside;
+    if (mine) sh.tops[threadIdx.x] = logit_of((uint32_t)(own >> 32)), sh.sums[threadIdx.x] = sum, sh.held[threadIdx.x] = (uint32_t)(tail >> 32);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) outside = fmaxf(outside, sh.wave_float[i]);
+
+    // the row's sum, in units of its best token
+    double part = 0.0;
+    if (mine) part = sum * (double)scale.e(sh.tops[threadIdx.x], top);
+    double row_sum;
+    block_before(part, sh.wave_sum, &row_sum);
+    uint32_t token;
+    double kept;   // weight of the kept tokens in units of the best one
+    const Cut all{0, kAll};
+    // The token of the row, thread c holding the kept weight of chunk c (and the ties of earlier ones): the chunk in
+    // which the running sum passes uniform * sum, then the token in it.
+    auto pick = [&](double part, Cut cut, uint32_t ties_before, double* sum) LS_INLINE -> uint32_t {
+        __syncthreads();
+        const double before = block_before(part, sh.wave_sum, sum);
+        const float u = a.uniform[r] > 0.0f ? fminf(a.uniform[r], 1.0f) : 0.0f;
+        const double target = fmin((double)u * *sum, *sum * (1.0 - 0x1p-52));
+        if (threadIdx.x == 0) sh.token = 0;
+        __syncthreads();
+        // the last chunk with weight that starts at or before the target
+        if (mine && part > 0.0 && before <= target) atomicMax(&sh.token, threadIdx.x);
+        __syncthreads();
+        const uint32_t chunk = sh.token;
+        if (threadIdx.x == chunk) sh.wave_sum[0] = target - before, sh.before_count = ties_before;
+        __syncthreads();
+        const double rest = sh.wave_sum[0];
+        ties_before = sh.before_count;
+        __syncthreads();
+        return draw_from_chunk<T, kChunk>(logits, a.vocab, chunk, top, scale, cut, ties_before, rest, sh);
+    };
+
+    if (!by_count && !by_weight && !(min_p > 0.0f)) {
+        token = pick(part, all, 0, &kept);
+    } else {
+        // ---- candidates, in order of id: slots thread * kSlots + i
+        constexpr uint32_t kSlots = kCandidates / kThreads;
+        uint32_t order[kSlots], id[kSlots], weight[kSlots];
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) {
+            const uint32_t slot = threadIdx.x * kSlots + i, chunk = slot / rows.room, at = slot % rows.room;
+            uint64_t x = 0;
+            if (chunk < rows.chunks && at < sh.held[chunk]) x = get(record + chunk * words + sizeof(Record) / 8 + at);
+            order[i] = (uint32_t)(x >> 32);
+            id[i] = (uint32_t)x;
+            weight[i] = x ? scale.weight(logit_of(order[i]), top) : 0;
+        }
+        // what is no candidate does not matter if it weighs nothing
+        const uint32_t edge = outside > -INFINITY && scale.weight(outside, top) ? order_of(outside) : 0;
+        auto candidates = [&](auto f) LS_INLINE {
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i) f(order[i], weight[i]);
+        };
+        auto everything = [&](auto f) LS_INLINE {
+            for (uint32_t i = threadIdx.x; i < a.vocab; i += kThreads) {
+                const float v = to_float(logits[i]);
+                f(order_of(v), v > -INFINITY ? scale.weight(v, top) : 0u);
+            }
+        };
+        auto above = [edge](Cut x) { return x.order > edge || !edge; };
+        Cut cut = all;
+        uint64_t total = (uint64_t)(row_sum * 4294967296.0);
+        bool known = by_count || by_weight || !edge;   // every kept token is a candidate
+        if (by_count) {
+            cut = select(candidates, cut, (uint32_t)top_k, ~0ull, sh, &total);
+            known = above(cut);
+        }
+        const bool open = !known && by_weight;   // the weight that top-p takes its share of is not known
+        if (by_weight && known) {
+            const uint64_t limit = share(total, top_p, true);
+            cut = select(candidates, cut, kAll, limit ? limit : 1, sh, &total);
+            known = above(cut);
+        }
+        // Where the cut lies below, min-p may still leave out whatever is no candidate: it then decides alone.
+        if (!known && !open && !(scale.e(outside, top) >= min_p)) known = true, cut = all;
+        // Top-p by the chunks' bins: false where the bin of the cut holds more tokens than there are slots, or where
+        // min-p cuts above it.
+        double bin_kept = 0.0;
+        auto cut_in_bins = [&]() LS_INLINE -> bool {
+            const int row_bin = scale.bin(top);
+            const double limit = (double)fmaxf(top_p, 0.0f) * row_sum;
+            // thread b: bin b of the row, chunk by chunk
+            uint32_t n = 0;
+            double w = 0.0;
+            for (uint32_t c = 0; c < rows.chunks; ++c) {
+                const int b = (int)threadIdx.x - (row_bin - scale.bin(sh.tops[c]));
+                if (!(sh.tops[c] > -INFINITY) || b < 0) continue;
+                const uint64_t x = get(record + c * words + sizeof(Record) / 8 + rows.room + b);
+                n += (uint32_t)(x >> kCountShift);
+                w += (double)(x & ((1ull << kCountShift) - 1)) * 0x1p-32 * (double)scale.e(sh.tops[c], top);
+            }
+            double all_bins;
+            __syncthreads();
+            const double before = block_before(w, sh.wave_sum, &all_bins);
+            if (threadIdx.x == 0) sh.token = kAll, sh.turn = 0;
+            __syncthreads();
+            if (n && before < limit && before + w >= limit) atomicMin(&sh.token, threadIdx.x);
+            __syncthreads();
+            const uint32_t bin = sh.token;
+            if (bin == kAll) return false;
+            if (threadIdx.x == bin) sh.before_weight = (uint64_t)((limit - before) * 4294967296.0), sh.before_count = n;
+            __syncthreads();
+            if (sh.before_count > kCandidates) return false;
+            const uint64_t need = sh.before_weight;
+            // its tokens, in any order, into the slots of the candidates (which are all read)
+            const int wanted = row_bin - (int)bin;
+            auto slot_at = [&](uint32_t slot) { return record + slot / rows.room * words + sizeof(Record) / 8 + slot % rows.room; };
+            auto take = [&](float v, uint32_t i) LS_INLINE {
+                if (v > -INFINITY && scale.bin(v) == wanted) {
+                    const uint32_t slot = atomicAdd(&sh.turn, 1u);
+                    if (slot < rows.room * rows.chunks) put(slot_at(slot), (uint64_t)order_of(v) << 32 | i);
+                }
+            };
+            const uint32_t whole = a.vocab / 8;
+#pragma unroll 4
+            for (uint32_t i = threadIdx.x; i < whole; i += kThreads) {
+                const typename Vec8<T>::type x = *(const typename Vec8<T>::type*)(logits + 8 * i);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) take(to_float(x[j]), 8 * i + j);
+            }
+            if (8 * whole + threadIdx.x < a.vocab) take(to_float(logits[8 * whole + threadIdx.x]), 8 * whole + threadIdx.x);
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            __builtin_amdgcn_s_waitcnt(0);
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            __syncthreads();
+            const uint32_t held = sh.turn;
+            if (held > rows.room * rows.chunks) return false;
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i) {
+                const uint32_t slot = threadIdx.x * kSlots + i;
+                const uint64_t x = slot < held ? get(slot_at(slot)) : 0;
+                order[i] = (uint32_t)(x >> 32);
+                id[i] = (uint32_t)x;
+                weight[i] = x ? scale.weight(logit_of(order[i]), top) : 0;
+            }
+            uint64_t of_list;
+            cut = select(candidates, all, kAll, need ? need : 1, sh, &of_list);
+            if (!cut.order) {   // not reached, by a rounding of the bins' sums: all of the bin
+                if (threadIdx.x == 0) sh.token = kAll;
+                __syncthreads();
+                candidates([&](uint32_t o, uint32_t w) LS_INLINE {
+                    if (w) atomicMin(&sh.token, o);
+                });
+                __syncthreads();
+                cut = Cut{sh.token, kAll};
+                if (sh.token == kAll) return false;
+            }
+            if (min_p > 0.0f && !(scale.e(logit_of(cut.order), top) >= min_p)) return false;
+            // kept weight of every chunk: its bins above, and what the list holds of it
+            __syncthreads();
+            if (threadIdx.x < rows.chunks) sh.list[threadIdx.x] = 0, sh.held[threadIdx.x] = 0;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i) {
+                if (weight[i] && order[i] > cut.order) atomicAdd((unsigned long long*)&sh.list[id[i] / kChunk], (unsigned long long)weight[i]);
+                if (weight[i] && order[i] == cut.order) atomicAdd(&sh.held[id[i] / kChunk], 1u);
+            }
+            for (uint32_t c = wave; c < rows.chunks; c += kWaves) {
+                const float ctop = sh.tops[c];
+                double x = 0.0;
+                if (ctop > -INFINITY) {
+                    const uint64_t* bins = record + c * words + sizeof(Record) / 8 + rows.room;
+                    const int shift = row_bin - scale.bin(ctop);
+                    for (int b = (int)lane; b < (int)bin - shift; b += 64) x += (double)(get(bins + b) & ((1ull << kCountShift) - 1));
+                    x *= 0x1p-32 * (double)scale.e(ctop, top);
+                }
+#pragma unroll
+                for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+                if (lane == 0) sh.sums[c] = x;
+            }
+            __syncthreads();
+            const uint32_t ties = mine ? sh.held[threadIdx.x] : 0;
+            uint32_t all_ties;
+            const uint32_t ties_before = block_before(ties, sh.wave32, &all_ties);
+            double part = 0.0;
+            if (mine) {
+                const uint32_t admitted = min(ties, cut.ties - min(cut.ties, ties_before));
+                part = sh.sums[threadIdx.x] +
+                       (double)(sh.list[threadIdx.x] + (uint64_t)admitted * scale.weight(logit_of(cut.order), top)) * 0x1p-32;
+            }
+            token = pick(part, cut, ties_before, &bin_kept);
+            return true;
+        };
+        uint64_t sum64;
+        if (known) {
+            uint32_t ties = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i) {
+                if (order[i] < cut.order || !(scale.e(logit_of(order[i]), top) >= min_p)) weight[i] = 0;
+                ties += weight[i] && order[i] == cut.order;
+            }
+            uint32_t all_ties;
+            __syncthreads();
+            uint32_t tie = block_before(ties, sh.wave32, &all_ties);
+            uint64_t thread_sum = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i) {
+                if (weight[i] && order[i] == cut.order && tie++ >= cut.ties) weight[i] = 0;
+                thread_sum += weight[i];
+            }
+            unsigned long long kept_sum;
+            uint64_t before = block_before((unsigned long long)thread_sum, (unsigned long long*)sh.wave64, &kept_sum);
+            sum64 = kept_sum;
+            const uint64_t target = min(share(sum64, a.uniform[r], false), sum64 - 1);
+            if (target >= before && target < before + thread_sum) {
+#pragma unroll
+                for (uint32_t i = 0; i < kSlots; ++i) {
+                    if (weight[i] && target >= before && target < before + weight[i]) sh.token = id[i];
+                    before += weight[i];
+                }
+            }
+            __syncthreads();
+            token = sh.token;
+            kept = (double)sum64 * 0x1p-32;
+        } else if (binned && cut_in_bins()) {
+            kept = bin_kept;
+        } else {
+            cut = all;
+            if (by_count || by_weight) cut = select(everything, cut, by_count ? (uint32_t)top_k : kAll, ~0ull, sh, &total);
+            if (by_weight) {
+                const uint64_t limit = share(total, top_p, true);
+                cut = select(everything, cut, kAll, limit ? limit : 1, sh, &total);
+            }
+            draw_from_row(logits, a.vocab, top, scale, cut, min_p, a.uniform[r], sh, &token, &sum64);
+            kept = (double)sum64 * 0x1p-32;
+        }
+    }
+    if (threadIdx.x == 0) {
+        a.tokens[r] = (int32_t)token;
+        // from the exponent itself: a small weight's rounding does not show in its logarithm
+        const float v = to_float(logits[token]);
+        if (a.logprob) a.logprob[r] = (v == top ? 0.0f : (v - top) / temperature) - (float)log(kept);
     }
 }
 
@@ -249,20 +757,60 @@ int check(const ls_hip_sample& a) {
     return 0;
 }
 
+// Chunks of 4096 logits while the rows are few (less than one workgroup a compute unit with twice as many),
+// of 8192 otherwise; a row's candidates are shared out evenly.
+RowArgs plan_rows(const ls_hip_sample& a, int* vecs) {
+    RowArgs p{};
+    const uint32_t twice = (a.vocab + 16 * kThreads - 1) / (16 * kThreads);
+    *vecs = a.vocab <= 64 * 8 * kThreads && (uint64_t)a.rows * twice < 256 ? 1 : 2;
+    const uint32_t chunk = 8 * *vecs * kThreads;
+    p.chunks = (a.vocab + chunk - 1) / chunk;
+    p.room = std::min(kCandidates / p.chunks, kChunkCandidates);
+    p.words = sizeof(Record) / 8 + p.room + kBins;
+    return p;
+}
+
+template <class T>
+void launch(ls_hip_sample a, hipStream_t st) {
+    int vecs;
+    const RowArgs p = plan_rows(a, &vecs);
+    const uint32_t rows = a.rows;
+    for (uint32_t r = 0; r < rows; r += kRowBlock) {
+        const dim3 grid(p.chunks, std::min(rows - r, kRowBlock));
+        if (vecs == 1) sample_kernel<T, 1><<<grid, kThreads, 0, st>>>(a, p);
+        else sample_kernel<T, 2><<<grid, kThreads, 0, st>>>(a, p);
+        a.logits = (const T*)a.logits + (int64_t)kRowBlock * a.row_stride;
+        a.uniform += kRowBlock;
+        a.tokens += kRowBlock;
+        if (a.temperature) a.temperature += kRowBlock;
+        if (a.top_k) a.top_k += kRowBlock;
+        if (a.top_p) a.top_p += kRowBlock;
+        if (a.min_p) a.min_p += kRowBlock;
+        if (a.logprob) a.logprob += kRowBlock;
+    }
+}
+
 }  // namespace
 }  // namespace lsamd
 
-extern "C" uint64_t ls_hip_sample_workspace(const ls_hip_sample*) { return 0; }
+extern "C" uint64_t ls_hip_sample_workspace(const ls_hip_sample* a) {
+    using namespace lsamd;
+    if (!a || check(*a) || !a->rows) return 0;
+    int vecs;
+    const RowArgs p = plan_rows(*a, &vecs);
+    return kCounterBytes + (uint64_t)std::min(a->rows, kRowBlock) * p.chunks * p.words * 8ull;
+}
 
 extern "C" int ls_hip_sample_enqueue(const ls_hip_sample* a, void* stream) {
     using namespace lsamd;
     if (!a) return EINVAL;
     if (const int rc = check(*a)) return rc;
     if (!a->rows) return 0;
+    if (!a->workspace || a->workspace_bytes < ls_hip_sample_workspace(a)) return ENOSPC;
     const auto st = static_cast<hipStream_t>(stream);
-    if (a->dtype == LS_TYPE_F16) sample_kernel<_Float16><<<a->rows, kThreads, 0, st>>>(*a);
-    else if (a->dtype == LS_TYPE_BF16) sample_kernel<__bf16><<<a->rows, kThreads, 0, st>>>(*a);
-    else sample_kernel<float><<<a->rows, kThreads, 0, st>>>(*a);
+    if (a->dtype == LS_TYPE_F16) launch<_Float16>(*a, st);
+    else if (a->dtype == LS_TYPE_BF16) launch<__bf16>(*a, st);
+    else launch<float>(*a, st);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : static_cast<int>(e);
 }

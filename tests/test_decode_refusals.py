@@ -5,7 +5,7 @@ import pytest
 
 from leanstream_amd import _native
 
-EINVAL, ENOTSUP = 22, 95
+EINVAL, ENOTSUP, ENOSPC = 22, 95, 28
 NAN, INF = float("nan"), float("inf")
 
 
@@ -41,6 +41,7 @@ def sample(**kw):
     return _native.Sample(**f)
 
 
+LONG = dict(max_context=16384, table_width=1024, table_stride=1024)
 CASES = [
     ("attention", attention, [
         (dict(q=None), EINVAL), (dict(out=None), EINVAL), (dict(k_pages=None), EINVAL), (dict(context=None), EINVAL),
@@ -49,7 +50,9 @@ CASES = [
         (dict(max_new=5), EINVAL), (dict(table_stride=7), EINVAL), (dict(scale=NAN), EINVAL), (dict(scale=INF), EINVAL),
         (dict(q=0x1008), EINVAL), (dict(out=0x1002), EINVAL), (dict(workspace=0x1004), EINVAL),
         (dict(q_head_stride=132), EINVAL), (dict(v_slot_stride=-128), EINVAL), (dict(dtype=3), EINVAL),
-        (dict(window=0x40000000), EINVAL), (dict(dtype=2), ENOTSUP), (dict(head_dim=96), ENOTSUP)]),
+        (dict(window=0x40000000), EINVAL), (dict(dtype=2), ENOTSUP), (dict(head_dim=96), ENOTSUP),
+        (dict(k_slot_stride=1 << 27), ENOTSUP), (dict(LONG), ENOSPC),
+        (dict(LONG, workspace=0x1000, workspace_bytes=64), ENOSPC)]),
     ("append", append, [
         (dict(k=None), EINVAL), (dict(v_pages=None), EINVAL), (dict(q=None), EINVAL), (dict(q_out=None), EINVAL),
         (dict(cos=None), EINVAL), (dict(positions=0), EINVAL), (dict(rot=130), EINVAL), (dict(rot=127), EINVAL),
@@ -63,7 +66,8 @@ CASES = [
     ("sample", sample, [
         (dict(logits=None), EINVAL), (dict(uniform=None), EINVAL), (dict(tokens=None), EINVAL), (dict(vocab=0), EINVAL),
         (dict(dtype=3), EINVAL), (dict(logits=0x1002), EINVAL), (dict(tokens=0x1001), EINVAL),
-        (dict(row_stride=-1), EINVAL), (dict(vocab=(1 << 20) + 1), ENOTSUP)]),
+        (dict(row_stride=-1), EINVAL), (dict(workspace=0x1008), EINVAL), (dict(vocab=(1 << 20) + 1), ENOTSUP),
+        (dict(), ENOSPC), (dict(workspace=0x1000, workspace_bytes=64), ENOSPC)]),
 ]
 
 

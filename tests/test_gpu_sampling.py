@@ -235,3 +235,21 @@ def test_in_a_graph_and_on_another_stream(torch_gpu):
         call.enqueue(side.cuda_stream)
         torch.cuda.synchronize()
         assert torch.equal(tokens, want)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("vocab", [3000, 20000, 60001, 131072])
+def test_wide_nuclei(torch_gpu, vocab, dtype):
+    """Rows without outstanding tokens: top-p keeps thousands (in bf16 many of them equal), with and without a
+    min-p that keeps fewer; top-k beyond what a chunk remembers."""
+    torch = torch_gpu
+    rows = 12
+    logits, u, g = random_rows(torch, rows, vocab, dtype, vocab + 1, peaks=1, spread=1.0)
+    p = [0.2, 0.5, 0.8, 0.9, 0.95, 0.99, 0.999, 0.3, 0.6, 0.7, 0.97, 0.9]
+    check(torch, logits, u, None, None, p)
+    check(torch, logits, u, [3.0] * rows, None, p)
+    check(torch, logits, u, [0.2, 0.5, 1.7, 30.0] * 3, None, p)
+    check(torch, logits, u, [2.0] * rows, None, p, [0.001, 0.05, 0.3] * 4)
+    check(torch, logits, u, [2.0] * rows, [2999, 1500, 700] * 4, p)
+    check(torch, logits, u, [2.0] * rows, [2999, 1500, 700] * 4)
+    check(torch, logits, u, [2.0] * rows, None, None, [0.001, 0.05, 0.3] * 4)
