@@ -4,10 +4,10 @@
 // kept tokens are a prefix of the ranking: everything above a cut logit, and of the tokens equal to it the
 // first few by id. Weights of a set are summed as whole numbers, so no order of atomics changes a result.
 //
-// One pass over the logits: a workgroup takes a chunk of a row and leaves its best token, the sum of its
-// exponentials and, in order of id, its candidates: as many of its largest logits as the record holds. The
-// workgroup that finishes a row last finds the cuts of top-k and of top-p among the candidates by radix
-// selection (8 bits of the logits' 32-bit order at a time, with the count and the weight of every digit).
+// One pass over the logits, in two launches. A workgroup of the first takes a chunk of a row and leaves its best token, the sum of its
+// exponentials and, in order of id, its candidates: as many of its largest logits as the record holds. A workgroup of
+// the second takes a row: it finds the cuts of top-k and of top-p among the candidates by radix
+// selection (parts of the range of their 32-bit order, with the count and the weight of each).
 // Whatever lies above the largest logit that is no candidate (`outside`) is known completely. Where a cut falls
 // below:
 //  - top-p alone: the chunks also left histograms of count and weight over bins of T / 16. They name the bin of
@@ -36,7 +36,6 @@ constexpr uint32_t kChunkCandidates = 256; // of a chunk, at most
 constexpr uint32_t kRowBlock = 256;        // rows of a launch
 constexpr int kBins = 512;                 // steps of T / 16 down from a chunk's best logit: weights to e^-32
 constexpr int kCountShift = 46;            // a bin: count << 46 | weight (at most 2^13 tokens of up to 2^32)
-constexpr uint64_t kCounterBytes = kRowBlock * sizeof(uint32_t);
 constexpr uint32_t kAll = 0xffffffffu;
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -80,10 +79,11 @@ struct Scale {
         // equal also where both are infinite; NaN (-inf at an infinite temperature, an infinite scale) became 0
         return l == top ? ldexpf(1.0f, up) : x;
     }
-    // weight in steps of 2^-32; the best token's 2^32 is held as 2^32 - 1
-    __device__ __forceinline__ uint32_t weight(float l, float top) const {
-        return (uint32_t)fminf(rintf(e(l, top, 32)), 4294967040.0f) | (l == top ? 255u : 0u);
+    // weight in steps of 2^-32 from e 2^32; the best token's 2^32 is held as 2^32 - 1
+    static __device__ __forceinline__ uint32_t weight_of(float e, bool best) {
+        return (uint32_t)fminf(rintf(e), 4294967040.0f) | (best ? 255u : 0u);
     }
+    __device__ __forceinline__ uint32_t weight(float l, float top) const { return weight_of(e(l, top, 32), l == top); }
 };
 
 // A prefix of the ranking: every order above `order`, and the first `ties` ids of those equal to it.
@@ -105,7 +105,13 @@ struct Shared {
     uint64_t list[kMaxChunks];
     float tops[kMaxChunks];
     uint32_t held[kMaxChunks];
+    uint64_t few[64];
+};
+struct ChunkShared {
     uint64_t bins[kBins];
+    double wave_sum[kWaves];
+    float wave_float[kWaves], wave_mean[kWaves];
+    uint32_t wave32[kWaves], digit;
 };
 
 __device__ __forceinline__ uint64_t wave_max(uint64_t x) {
@@ -140,23 +146,28 @@ __device__ __forceinline__ V block_before(V x, V* scratch, V* total) {
 }
 
 // The shortest prefix within `limit` whose count reaches need_count or whose weight reaches need_weight, of the
-// tokens that each(f) hands to f(order, weight); all of `limit` if none does. kept: the weight of that prefix.
+// tokens with an order in [base, high] that each(f) hands to f(order, weight); all of `limit` if none does.
+// kept: the weight of that prefix. A limit with fewer ties than there are must weigh need_weight. Every pass counts the 256 equal parts of the range and goes on with the one
+// in which a sum is reached, until it is one logit or holds so few tokens that one wave ranks them.
 template <class Each>
-__device__ __forceinline__ Cut select(const Each& each, Cut limit, uint32_t need_count, uint64_t need_weight, Shared& sh, uint64_t* kept) {
-    uint32_t prefix = 0;
+__device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t high, Cut limit, uint32_t need_count,
+                                      uint64_t need_weight, Shared& sh, uint64_t* kept) {
     uint64_t before_weight = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    base = max(base, limit.order);
+    for (;;) {
+        const int shift = max(0, 24 - __clz((int)((high - base) | 1)));
         __syncthreads();
         for (int i = threadIdx.x; i < 256; i += kThreads) sh.weights[i] = 0, sh.counts[i] = 0;
+        if (threadIdx.x == 0) sh.turn = 0;
         __syncthreads();
         each([&](uint32_t order, uint32_t weight) LS_INLINE {
-            if (!weight || order < limit.order || (shift < 24 && (order >> shift >> 8) != (prefix >> shift >> 8))) return;
-            atomicAdd(&sh.counts[order >> shift & 255], 1u);
-            atomicAdd((unsigned long long*)&sh.weights[order >> shift & 255], (unsigned long long)weight);
+            if (!weight || order < base || order > high) return;
+            atomicAdd(&sh.counts[(order - base) >> shift], 1u);
+            atomicAdd((unsigned long long*)&sh.weights[(order - base) >> shift], (unsigned long long)weight);
         });
         __syncthreads();
-        // The first digit from above at which one of the sums is reached: a lane takes four digits. At the last
-        // level a digit is one logit, and of the limit's own logit only its ties count.
+        // The first part from above at which one of the sums is reached: a lane takes four. Where a part is one
+        // logit, only its ties count of the limit's own.
         if (threadIdx.x < 64) {
             const uint32_t lane = threadIdx.x;
             uint32_t n[4], c = 0;
@@ -166,7 +177,7 @@ __device__ __forceinline__ Cut select(const Each& each, Cut limit, uint32_t need
                 const uint32_t d = 255 - 4 * lane - i;
                 n[i] = sh.counts[d];
                 w[i] = sh.weights[d];
-                if (shift == 0 && (prefix | d) == limit.order && n[i] > limit.ties) w[i] = w[i] / n[i] * limit.ties, n[i] = limit.ties;
+                if (shift == 0 && base + d == limit.order && n[i] > limit.ties) w[i] = w[i] / n[i] * limit.ties, n[i] = limit.ties;
                 c += n[i];
                 s += w[i];
             }
@@ -196,34 +207,55 @@ __device__ __forceinline__ Cut select(const Each& each, Cut limit, uint32_t need
             *kept = before_weight;
             return limit;
         }
-        prefix |= digit << shift;
+        uint32_t n = sh.counts[digit];
         if (shift == 0) {
-            uint32_t n = sh.counts[digit];
             const uint64_t one = sh.weights[digit] / n;
-            if (prefix == limit.order) n = min(n, limit.ties);
+            if (base + digit == limit.order) n = min(n, limit.ties);
             // ties needed for the count and for the weight, whichever is reached first
             const uint64_t ties = min(min((uint64_t)n, (uint64_t)need_count), (need_weight - 1) / one + 1);
             *kept = before_weight + ties * one;
-            return Cut{prefix, (uint32_t)ties};
+            return Cut{base + digit, (uint32_t)ties};
         }
+        base += digit << shift;
+        high = min(high, base + ((1u << shift) - 1));
+        if (n > 64) continue;
+        each([&](uint32_t order, uint32_t weight) LS_INLINE {
+            if (!weight || order < base || order > high) return;
+            const uint32_t i = atomicAdd(&sh.turn, 1u);
+            sh.few[i] = (uint64_t)order << 32 | weight;
+        });
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const uint64_t own = threadIdx.x < n ? sh.few[threadIdx.x] : 0;
+            const uint32_t order = (uint32_t)(own >> 32), weight = (uint32_t)own;
+            uint32_t c = 0, equal = 0;
+            uint64_t s = 0;
+            for (uint32_t i = 0; i < n; ++i) {
+                const uint32_t o = __builtin_amdgcn_readlane(order, i), w = __builtin_amdgcn_readlane(weight, i);
+                if (o > order) ++c, s += w;
+                equal += o == order;
+            }
+            if (order == limit.order) equal = min(equal, limit.ties);
+            const bool reached = weight && c < need_count && s < need_weight &&
+                                 (c + equal >= need_count || s + (uint64_t)equal * weight >= need_weight);
+            const uint64_t at = __ballot(reached);
+            if (threadIdx.x == (uint32_t)__ffsll((unsigned long long)at) - 1) {
+                const uint64_t ties = min(min((uint64_t)equal, (uint64_t)(need_count - c)), (need_weight - s - 1) / weight + 1);
+                sh.before_count = order;
+                sh.before_weight = s + ties * weight;
+                sh.turn = (uint32_t)ties;
+            }
+        }
+        __syncthreads();
+        *kept = before_weight + sh.before_weight;
+        return Cut{sh.before_count, sh.turn};
     }
-    return limit;
 }
 
-// What a chunk leaves for its row; the candidates (order << 32 | id) follow in order of id, then the bins.
-struct Record {
-    uint64_t best;        // order << 32 | ~id
-    double sum;           // of exp((l - top) / T), top the chunk's
-    float outside;        // the largest logit that is no candidate, -inf: none
-    uint32_t count;
-};
-
-__device__ __forceinline__ void put(uint64_t* p, uint64_t v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ uint64_t get(const uint64_t* p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
+// What a chunk leaves for its row, in 8-byte words: its best token (order << 32 | ~id), the sum of exp((l - top) /
+// T) with top the chunk's, the number of candidates and the largest logit that is none (-inf: there is none);
+// then the candidates (order << 32 | id) in order of id, then the bins.
+constexpr int kHead = 3;
 
 template <class T>
 struct Vec8 {
@@ -302,15 +334,24 @@ template <class T, uint32_t Chunk>
 __device__ __forceinline__ uint32_t draw_from_chunk(const T* logits, uint32_t vocab, uint32_t chunk, float top, const Scale& scale, Cut cut,
                                     uint32_t ties_before, double rest, Shared& sh) {
     constexpr uint32_t kEach = Chunk / kThreads;
-    const uint32_t from = chunk * Chunk, to = min(from + Chunk, vocab);
+    const uint32_t from = chunk * Chunk + threadIdx.x * kEach;
     float x[kEach];
     uint32_t o[kEach], ties = 0;
 #pragma unroll
+    for (uint32_t v = 0; v < kEach; v += 8) {
+        if (from + v + 8 <= vocab) {
+            const typename Vec8<T>::type y = *(const typename Vec8<T>::type*)(logits + from + v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[v + j] = to_float(y[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[v + j] = from + v + j < vocab ? to_float(logits[from + v + j]) : -INFINITY;
+        }
+    }
+#pragma unroll
     for (uint32_t j = 0; j < kEach; ++j) {
-        const uint32_t i = from + threadIdx.x * kEach + j;
-        const float v = i < to ? to_float(logits[i]) : -INFINITY;
-        o[j] = order_of(v);
-        x[j] = v > -INFINITY && o[j] >= cut.order ? scale.e(v, top) : 0.0f;
+        o[j] = order_of(x[j]);
+        x[j] = x[j] > -INFINITY && o[j] >= cut.order ? scale.e(x[j], top) : 0.0f;
         ties += o[j] == cut.order;
     }
     uint32_t chunk_ties;
@@ -324,40 +365,69 @@ __device__ __forceinline__ uint32_t draw_from_chunk(const T* logits, uint32_t vo
     double chunk_sum;
     double before = block_before(thread_sum, sh.wave_sum, &chunk_sum);
     // `rest` and these sums are rounded apart: the last token with weight takes what is left
-    if (threadIdx.x == 0) sh.token = kAll, sh.digit = 0;
-    __syncthreads();
+    uint32_t first = kAll, last = 0;
 #pragma unroll
     for (uint32_t j = 0; j < kEach; ++j) {
-        const uint32_t i = from + threadIdx.x * kEach + j;
         before += x[j];
         if (x[j] > 0.0f) {
-            if (before > rest) atomicMin(&sh.token, i);
-            atomicMax(&sh.digit, i);
+            if (before > rest) first = min(first, from + j);
+            last = from + j;
         }
     }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        first = min(first, (uint32_t)__shfl_xor(first, d));
+        last = max(last, (uint32_t)__shfl_xor(last, d));
+    }
     __syncthreads();
-    return min(sh.token, sh.digit);
+    if ((threadIdx.x & 63) == 0) sh.wave32[threadIdx.x >> 6] = first, sh.wave64[threadIdx.x >> 6] = last;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        first = min(first, sh.wave32[i]);
+        last = max(last, (uint32_t)sh.wave64[i]);
+    }
+    return min(first, last);
 }
 
+// A row's settings.
+struct Settings {
+    float temperature, top_p, min_p;
+    uint32_t top_k;
+    bool greedy, by_count, by_weight;
+    bool filtered;   // by count, weight or chance
+    bool summed;     // needs the sum of all exponentials
+    bool binned;     // may need the histograms
+    __device__ __forceinline__ Settings(const ls_hip_sample& a, uint32_t r) {
+        temperature = a.temperature ? a.temperature[r] : 1.0f;
+        const int32_t k = a.top_k ? a.top_k[r] : 0;
+        top_k = k > 0 ? (uint32_t)k : kAll;
+        top_p = a.top_p ? a.top_p[r] : 1.0f;
+        min_p = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
+        greedy = !(temperature > 0.0f);
+        if (greedy) temperature = 1.0f;
+        by_count = top_k < a.vocab;
+        by_weight = top_p < 1.0f;
+        filtered = !greedy && (by_count || by_weight || min_p > 0.0f);
+        summed = !greedy && !by_count && (by_weight || !filtered);
+        binned = summed && by_weight;
+    }
+};
+
 template <class T, int Vecs>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a, const RowArgs rows) {
+__global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sample a, const RowArgs rows) {
     constexpr uint32_t kChunk = 8 * Vecs * kThreads;
-    __shared__ Shared sh;
+    __shared__ ChunkShared sh;
     __shared__ __align__(16) uint8_t marks[kChunk / 8];
     const uint32_t r = blockIdx.y, c = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T* logits = (const T*)a.logits + (int64_t)r * a.row_stride;
     const uint32_t begin = c * kChunk, size = min(a.vocab - begin, kChunk);
-    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
-    const bool greedy = !(temperature > 0.0f);
-    const Scale scale(greedy ? 1.0f : temperature);
-    const int32_t top_k = a.top_k ? a.top_k[r] : 0;
-    const float top_p = a.top_p ? a.top_p[r] : 1.0f, min_p = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
-    const bool by_count = top_k > 0 && (uint32_t)top_k < a.vocab, by_weight = top_p < 1.0f;
-    const bool binned = by_weight && !by_count;   // may need the histograms
+    const Settings set(a, r);
+    const bool greedy = set.greedy, filtered = set.filtered, summed = set.summed, binned = set.binned;
+    const Scale scale(set.temperature);
 
-    // ---- the chunk: element 8 (v kThreads + thread) + j
-    float l[Vecs][8];
-    uint64_t best = 0;
+    // element 8 (v kThreads + thread) + j
+    float l[Vecs][8], high = -INFINITY;
 #pragma unroll
     for (int v = 0; v < Vecs; ++v) {
         const uint32_t i = 8 * (v * kThreads + threadIdx.x);
@@ -374,22 +444,42 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
 #pragma unroll
     for (int v = 0; v < Vecs; ++v)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t id = begin + 8 * (v * kThreads + threadIdx.x) + j;
-            best = max(best, (uint64_t)order_of(l[v][j]) << 32 | (uint32_t)~id);
-        }
-    best = wave_max(best);
-    if (lane == 0) sh.wave64[wave] = best;
-    __syncthreads();
+        for (int j = 0; j < 8; ++j) high = fmaxf(high, l[v][j]);
+    // the best logit, and the mean of the threads' best ones: few logits of a chunk lie above that
+    float chunk_top = high, mean = high > -INFINITY ? high : 0.0f, some = high > -INFINITY ? 1.0f : 0.0f;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) best = max(best, sh.wave64[i]);
-    const float chunk_top = logit_of((uint32_t)(best >> 32));
+    for (int d = 32; d; d >>= 1) {
+        chunk_top = fmaxf(chunk_top, __shfl_xor(chunk_top, d));
+        mean += __shfl_xor(mean, d);
+        some += __shfl_xor(some, d);
+    }
+    if (lane == 0) sh.wave_float[wave] = chunk_top, sh.wave_mean[wave] = mean, sh.wave32[wave] = (uint32_t)some;
+    __syncthreads();
+    mean = 0.0f, some = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        chunk_top = fmaxf(chunk_top, sh.wave_float[i]);
+        mean += sh.wave_mean[i];
+        some += (float)sh.wave32[i];
+    }
+    mean /= some;
+    if (!(mean < chunk_top)) mean = -INFINITY;   // all alike, infinite or none: any
+    uint32_t best_at = kAll;
+    if (high == chunk_top)   // its lowest id
+#pragma unroll
+        for (int v = 0; v < Vecs; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (l[v][j] == chunk_top) best_at = min(best_at, begin + 8 * (v * kThreads + threadIdx.x) + j);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) best_at = min(best_at, (uint32_t)__shfl_xor(best_at, d));
+    __syncthreads();
+    if (lane == 0) sh.wave32[wave] = best_at;
 
-    uint64_t* record = (uint64_t*)((char*)a.workspace + kCounterBytes) +
-                       ((uint64_t)r * rows.chunks + c) * rows.words;
-    double sum = 0.0;
+    uint64_t* record = (uint64_t*)a.workspace + ((uint64_t)r * rows.chunks + c) * rows.words;
     const int top_bin = scale.bin(chunk_top);
-    if (!greedy) {
+    double sum = 0.0;
+    if (summed) {
         float mine = 0.0f;
 #pragma unroll
         for (int v = 0; v < Vecs; ++v)
@@ -397,20 +487,39 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
             for (int j = 0; j < 8; ++j) {
                 const float x = l[v][j];
                 if (!(x > -INFINITY)) continue;
-                mine += scale.e(x, chunk_top);
+                const float e = scale.e(x, chunk_top, 32);
+                mine += e;
                 const int down = top_bin - scale.bin(x);
-                if (down < kBins)
-                    atomicAdd((unsigned long long*)&sh.bins[down], 1ull << kCountShift | scale.weight(x, chunk_top));
+                if (binned && down < kBins)
+                    atomicAdd((unsigned long long*)&sh.bins[down], 1ull << kCountShift | scale.weight_of(e, x == chunk_top));
             }
-        sum = mine;
+        sum = (double)mine * 0x1p-32;
 #pragma unroll
         for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
         if (lane == 0) sh.wave_sum[wave] = sum;
-        __syncthreads();
+    } else if (!greedy && filtered) {
+#pragma unroll
+        for (int v = 0; v < Vecs; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = l[v][j];
+                const int down = top_bin - scale.bin(x);
+                if (x > mean && down < kBins) atomicAdd((unsigned long long*)&sh.bins[down], 1ull << kCountShift);
+            }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) best_at = min(best_at, sh.wave32[i]);
+    const uint64_t best_of_chunk = (uint64_t)order_of(chunk_top) << 32 | (uint32_t)~best_at;
+    if (summed) {
         sum = 0.0;
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) sum += sh.wave_sum[i];
-        // bins that fit into the record, as many as possible
+        if (threadIdx.x == 0) record[1] = __builtin_bit_cast(uint64_t, sum);
+    }
+    if (!greedy && filtered) {
+        // bins that fit into the record, as many as possible; where only what exceeds the mean was counted, the bins
+        // wholly above it
         if (wave == 0) {
             uint32_t n = 0, fit = 0;
 #pragma unroll
@@ -419,12 +528,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
 #pragma unroll
             for (int i = 0; i < kBins / 64; ++i) fit += (upto += (uint32_t)(sh.bins[kBins / 64 * lane + i] >> kCountShift)) <= rows.room;
             fit = __shfl(wave_upto(fit), 63);
-            if (lane == 0) sh.digit = fit;
+            if (lane == 0) sh.digit = summed || mean == -INFINITY ? fit : min(fit, (uint32_t)max(0, min(top_bin - scale.bin(mean), kBins)));
         }
         __syncthreads();
         const int bins = (int)sh.digit;
         if (binned)
-            for (int i = threadIdx.x; i < kBins; i += kThreads) put(record + sizeof(Record) / 8 + rows.room + i, sh.bins[i]);
+            for (int i = threadIdx.x; i < kBins; i += kThreads) record[kHead + rows.room + i] = sh.bins[i];
         float outside = -INFINITY;
 #pragma unroll
         for (int v = 0; v < Vecs; ++v) {
@@ -450,45 +559,33 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
         while (word) {
             const uint32_t id = begin + 32 * threadIdx.x + __ffs(word) - 1;
             word &= word - 1;
-            put(record + sizeof(Record) / 8 + at++, (uint64_t)order_of(to_float(logits[id])) << 32 | id);
+            record[kHead + at++] = (uint64_t)order_of(to_float(logits[id])) << 32 | id;
         }
-        if (threadIdx.x == 0) {
-            put(record + 1, __builtin_bit_cast(uint64_t, sum));
-            put(record + 2, (uint64_t)total << 32 | __float_as_uint(outside));
-        }
+        if (threadIdx.x == 0) record[2] = (uint64_t)total << 32 | __float_as_uint(outside);
     }
-    if (threadIdx.x == 0) put(record, best);
+    if (threadIdx.x == 0) record[0] = best_of_chunk;
+}
 
-    // ---- the row, by its last chunk. Every store of the workgroup has been acknowledged before its turn is taken.
-    if (rows.chunks > 1) {
-        __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        __builtin_amdgcn_s_waitcnt(0);
-        __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            uint32_t* counter = (uint32_t*)a.workspace + r;
-            sh.turn = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (sh.turn == rows.chunks - 1)   // ready for the next call
-                __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (sh.turn != rows.chunks - 1) return;
-    } else {
-        __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-    }
+template <class T, int Vecs>
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sample a, const RowArgs rows) {
+    constexpr uint32_t kChunk = 8 * Vecs * kThreads;
+    __shared__ Shared sh;
+    const uint32_t r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const T* logits = (const T*)a.logits + (int64_t)r * a.row_stride;
+    const Settings set(a, r);
+    const bool greedy = set.greedy, filtered = set.filtered, by_count = set.by_count, by_weight = set.by_weight;
+    const float top_p = set.top_p, min_p = set.min_p, temperature = set.temperature;
+    const Scale scale(temperature);
     const uint32_t words = rows.words;
-    record = (uint64_t*)((char*)a.workspace + kCounterBytes) + (uint64_t)r * rows.chunks * words;
+    uint64_t* record = (uint64_t*)a.workspace + (uint64_t)r * rows.chunks * words;
 
     // threads 0 .. chunks - 1 hold a record each; every thread takes some of the slots for candidates
     const bool mine = threadIdx.x < rows.chunks;
-    best = mine ? get(record + threadIdx.x * words) : 0;
-    uint64_t tail = mine && !greedy ? get(record + threadIdx.x * words + 2) : (uint64_t)__float_as_uint(-INFINITY);
-    sum = mine && !greedy ? __builtin_bit_cast(double, get(record + threadIdx.x * words + 1)) : 0.0;
+    uint64_t best = mine ? record[threadIdx.x * words] : 0;
+    const uint64_t tail = mine && filtered ? record[threadIdx.x * words + 2] : (uint64_t)__float_as_uint(-INFINITY);
+    const double sum = mine && set.summed ? __builtin_bit_cast(double, record[threadIdx.x * words + 1]) : 0.0;
     const uint64_t own = best;
     best = wave_max(best);
-    __syncthreads();
     if (lane == 0) sh.wave64[wave] = best;
     __syncthreads();
 #pragma unroll
@@ -541,7 +638,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
         return draw_from_chunk<T, kChunk>(logits, a.vocab, chunk, top, scale, cut, ties_before, rest, sh);
     };
 
-    if (!by_count && !by_weight && !(min_p > 0.0f)) {
+    if (!filtered) {
         token = pick(part, all, 0, &kept);
     } else {
         // ---- candidates, in order of id: slots thread * kSlots + i
@@ -551,12 +648,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
         for (uint32_t i = 0; i < kSlots; ++i) {
             const uint32_t slot = threadIdx.x * kSlots + i, chunk = slot / rows.room, at = slot % rows.room;
             uint64_t x = 0;
-            if (chunk < rows.chunks && at < sh.held[chunk]) x = get(record + chunk * words + sizeof(Record) / 8 + at);
+            if (chunk < rows.chunks && at < sh.held[chunk]) x = record[chunk * words + kHead + at];
             order[i] = (uint32_t)(x >> 32);
             id[i] = (uint32_t)x;
             weight[i] = x ? scale.weight(logit_of(order[i]), top) : 0;
         }
         // what is no candidate does not matter if it weighs nothing
+        // orders below this weigh nothing
+        const uint32_t low = order_of(top - 23.0f * temperature), high = order_of(top);
         const uint32_t edge = outside > -INFINITY && scale.weight(outside, top) ? order_of(outside) : 0;
         auto candidates = [&](auto f) LS_INLINE {
 #pragma unroll
@@ -573,13 +672,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
         uint64_t total = (uint64_t)(row_sum * 4294967296.0);
         bool known = by_count || by_weight || !edge;   // every kept token is a candidate
         if (by_count) {
-            cut = select(candidates, cut, (uint32_t)top_k, ~0ull, sh, &total);
+            cut = select(candidates, max(low, edge + 1), high, cut, set.top_k, ~0ull, sh, &total);
             known = above(cut);
         }
         const bool open = !known && by_weight;   // the weight that top-p takes its share of is not known
         if (by_weight && known) {
             const uint64_t limit = share(total, top_p, true);
-            cut = select(candidates, cut, kAll, limit ? limit : 1, sh, &total);
+            cut = select(candidates, max(low, edge + 1), high, cut, kAll, limit ? limit : 1, sh, &total);
             known = above(cut);
         }
         // Where the cut lies below, min-p may still leave out whatever is no candidate: it then decides alone.
@@ -596,7 +695,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
             for (uint32_t c = 0; c < rows.chunks; ++c) {
                 const int b = (int)threadIdx.x - (row_bin - scale.bin(sh.tops[c]));
                 if (!(sh.tops[c] > -INFINITY) || b < 0) continue;
-                const uint64_t x = get(record + c * words + sizeof(Record) / 8 + rows.room + b);
+                const uint64_t x = record[c * words + kHead + rows.room + b];
                 n += (uint32_t)(x >> kCountShift);
                 w += (double)(x & ((1ull << kCountShift) - 1)) * 0x1p-32 * (double)scale.e(sh.tops[c], top);
             }
@@ -615,11 +714,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
             const uint64_t need = sh.before_weight;
             // its tokens, in any order, into the slots of the candidates (which are all read)
             const int wanted = row_bin - (int)bin;
-            auto slot_at = [&](uint32_t slot) { return record + slot / rows.room * words + sizeof(Record) / 8 + slot % rows.room; };
+            auto slot_at = [&](uint32_t slot) { return record + slot / rows.room * words + kHead + slot % rows.room; };
             auto take = [&](float v, uint32_t i) LS_INLINE {
                 if (v > -INFINITY && scale.bin(v) == wanted) {
                     const uint32_t slot = atomicAdd(&sh.turn, 1u);
-                    if (slot < rows.room * rows.chunks) put(slot_at(slot), (uint64_t)order_of(v) << 32 | i);
+                    if (slot < rows.room * rows.chunks) *slot_at(slot) = (uint64_t)order_of(v) << 32 | i;
                 }
             };
             const uint32_t whole = a.vocab / 8;
@@ -630,22 +729,19 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
                 for (int j = 0; j < 8; ++j) take(to_float(x[j]), 8 * i + j);
             }
             if (8 * whole + threadIdx.x < a.vocab) take(to_float(logits[8 * whole + threadIdx.x]), 8 * whole + threadIdx.x);
-            __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            __builtin_amdgcn_s_waitcnt(0);
-            __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            __syncthreads();
+            __syncthreads();   // and their stores, for this workgroup
             const uint32_t held = sh.turn;
             if (held > rows.room * rows.chunks) return false;
 #pragma unroll
             for (uint32_t i = 0; i < kSlots; ++i) {
                 const uint32_t slot = threadIdx.x * kSlots + i;
-                const uint64_t x = slot < held ? get(slot_at(slot)) : 0;
+                const uint64_t x = slot < held ? *slot_at(slot) : 0;
                 order[i] = (uint32_t)(x >> 32);
                 id[i] = (uint32_t)x;
                 weight[i] = x ? scale.weight(logit_of(order[i]), top) : 0;
             }
             uint64_t of_list;
-            cut = select(candidates, all, kAll, need ? need : 1, sh, &of_list);
+            cut = select(candidates, low, high, all, kAll, need ? need : 1, sh, &of_list);
             if (!cut.order) {   // not reached, by a rounding of the bins' sums: all of the bin
                 if (threadIdx.x == 0) sh.token = kAll;
                 __syncthreads();
@@ -670,9 +766,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
                 const float ctop = sh.tops[c];
                 double x = 0.0;
                 if (ctop > -INFINITY) {
-                    const uint64_t* bins = record + c * words + sizeof(Record) / 8 + rows.room;
+                    const uint64_t* bins = record + c * words + kHead + rows.room;
                     const int shift = row_bin - scale.bin(ctop);
-                    for (int b = (int)lane; b < (int)bin - shift; b += 64) x += (double)(get(bins + b) & ((1ull << kCountShift) - 1));
+                    for (int b = (int)lane; b < (int)bin - shift; b += 64) x += (double)(bins[b] & ((1ull << kCountShift) - 1));
                     x *= 0x1p-32 * (double)scale.e(ctop, top);
                 }
 #pragma unroll
@@ -723,14 +819,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const ls_hip_sample a,
             __syncthreads();
             token = sh.token;
             kept = (double)sum64 * 0x1p-32;
-        } else if (binned && cut_in_bins()) {
+        } else if (set.binned && cut_in_bins()) {
             kept = bin_kept;
         } else {
             cut = all;
-            if (by_count || by_weight) cut = select(everything, cut, by_count ? (uint32_t)top_k : kAll, ~0ull, sh, &total);
+            if (by_count || by_weight) cut = select(everything, low, high, cut, by_count ? set.top_k : kAll, ~0ull, sh, &total);
             if (by_weight) {
                 const uint64_t limit = share(total, top_p, true);
-                cut = select(everything, cut, kAll, limit ? limit : 1, sh, &total);
+                cut = select(everything, low, high, cut, kAll, limit ? limit : 1, sh, &total);
             }
             draw_from_row(logits, a.vocab, top, scale, cut, min_p, a.uniform[r], sh, &token, &sum64);
             kept = (double)sum64 * 0x1p-32;
@@ -766,7 +862,7 @@ RowArgs plan_rows(const ls_hip_sample& a, int* vecs) {
     const uint32_t chunk = 8 * *vecs * kThreads;
     p.chunks = (a.vocab + chunk - 1) / chunk;
     p.room = std::min(kCandidates / p.chunks, kChunkCandidates);
-    p.words = sizeof(Record) / 8 + p.room + kBins;
+    p.words = kHead + p.room + kBins;
     return p;
 }
 
@@ -777,8 +873,13 @@ void launch(ls_hip_sample a, hipStream_t st) {
     const uint32_t rows = a.rows;
     for (uint32_t r = 0; r < rows; r += kRowBlock) {
         const dim3 grid(p.chunks, std::min(rows - r, kRowBlock));
-        if (vecs == 1) sample_kernel<T, 1><<<grid, kThreads, 0, st>>>(a, p);
-        else sample_kernel<T, 2><<<grid, kThreads, 0, st>>>(a, p);
+        if (vecs == 1) {
+            sample_chunk_kernel<T, 1><<<grid, kThreads, 0, st>>>(a, p);
+            sample_row_kernel<T, 1><<<grid.y, kThreads, 0, st>>>(a, p);
+        } else {
+            sample_chunk_kernel<T, 2><<<grid, kThreads, 0, st>>>(a, p);
+            sample_row_kernel<T, 2><<<grid.y, kThreads, 0, st>>>(a, p);
+        }
         a.logits = (const T*)a.logits + (int64_t)kRowBlock * a.row_stride;
         a.uniform += kRowBlock;
         a.tokens += kRowBlock;
@@ -798,7 +899,7 @@ extern "C" uint64_t ls_hip_sample_workspace(const ls_hip_sample* a) {
     if (!a || check(*a) || !a->rows) return 0;
     int vecs;
     const RowArgs p = plan_rows(*a, &vecs);
-    return kCounterBytes + (uint64_t)std::min(a->rows, kRowBlock) * p.chunks * p.words * 8ull;
+    return (uint64_t)std::min(a->rows, kRowBlock) * p.chunks * p.words * 8ull;
 }
 
 extern "C" int ls_hip_sample_enqueue(const ls_hip_sample* a, void* stream) {
