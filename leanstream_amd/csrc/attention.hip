@@ -33,6 +33,7 @@ constexpr float kNoKey = -1e30f;
 struct F16 {
     typedef half8 vec8;
     static constexpr uint32_t kExponent = 0x7c00u;   // all ones: infinity or NaN
+    static __device__ __forceinline__ float to_float(short x) { return (float)__builtin_bit_cast(_Float16, x); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         typedef _Float16 v2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, v2{(_Float16)a, (_Float16)b});
@@ -47,6 +48,7 @@ struct F16 {
 struct BF16 {
     typedef bhalf8 vec8;
     static constexpr uint32_t kExponent = 0x7f80u;
+    static __device__ __forceinline__ float to_float(short x) { return (float)__builtin_bit_cast(__bf16, x); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         typedef __bf16 v2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, v2{(__bf16)a, (__bf16)b});
@@ -59,6 +61,14 @@ struct BF16 {
     }
 };
 
+// Page tables and lengths do not change while a kernel runs: read through this view, uniform entries come over the
+// scalar cache and do not queue behind vector loads.
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef const __attribute__((address_space(4))) int32_t* Table;
+#else
+typedef const int32_t* Table;
+#endif
+
 struct Sequence {
     int first;    // its first row of q
     int tokens;   // new tokens
@@ -68,8 +78,8 @@ struct Sequence {
 // A sequence's lengths, held against the block's bounds: what lies outside has no tokens (their place in
 // q is unknown) or no keys.
 __device__ __forceinline__ Sequence read_sequence(const ls_hip_attention& a, int s) {
-    const int q0 = a.q_start[s], q1 = a.q_start[s + 1];
-    Sequence q{q0, q1 - q0, a.context[s]};
+    const int q0 = ((Table)a.q_start)[s], q1 = ((Table)a.q_start)[s + 1];
+    Sequence q{q0, q1 - q0, ((Table)a.context)[s]};
     bool bad = false;
     if (q0 < 0 || q1 < q0 || q1 > (int)a.tokens || (uint32_t)(q1 - q0) > a.max_new) {
         q.tokens = 0;
@@ -153,7 +163,7 @@ template <bool Large>
 struct StepPages {
     int page[Large ? 2 : 1];
     bool ok;   // no page out of range among them
-    __device__ __forceinline__ StepPages(const ls_hip_attention& a, const int32_t* table, int shift, int key0, int lane) {
+    __device__ __forceinline__ StepPages(const ls_hip_attention& a, Table table, int shift, int key0, int lane) {
         const int last = (int)a.table_width - 1;
         if constexpr (Large) {
             page[0] = table[min(key0 >> shift, last)];
@@ -217,7 +227,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
     f32x4 o[kLaneDims] = {};
     float m = kNoKey, l = 0.0f;
     const float scale = a.scale * kLog2e;
-    const int32_t* table = a.page_table + blockIdx.y * a.table_stride;
+    const Table table = (Table)(a.page_table + blockIdx.y * a.table_stride);
     const short* k_head = (const short*)a.k_pages + head * a.k_head_stride + 8 * g;
     const short* v_head = (const short*)a.v_pages + head * a.v_head_stride + kLaneDims * i16;
 
@@ -400,157 +410,350 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
 // ---------------------------------------------------------------------------------
 // Many rows
 // ---------------------------------------------------------------------------------
-constexpr int kTileWaves = 4;
-constexpr int kTileRows = 32 * kTileWaves;
-constexpr int kTileKeys = 64;
+// One workgroup: 4 waves of 32 * Halves rows of one sequence and KV head against all keys they see, Keys at a
+// time through LDS. Products are taken transposed, S^T = K Q^T and O^T = V^T P^T (32 x 32 x 16), so that a lane
+// holds scores of one row only and the P that it computed is already the second product's operand: key slots are
+// permuted alike in P and V^T, which a sum over keys allows. V^T comes out of LDS by transposing reads.
+//
+// Bound by the matrix cores, the exponentials close behind: the scores of the next tile are multiplied while
+// those of this one go through the softmax. Tiles come from memory without passing registers, two buffers each
+// of K and V, one barrier a tile.
+// The running maximum moves only where a score exceeds it by more than this (base 2): until then P is at most
+// 2^8 instead of 1, and the sums need no scaling.
+constexpr float kSlack = 8.0f;
 
-// One workgroup: 128 rows of one sequence and KV head against all keys they see, 64 at a time through LDS.
-// A wave owns 32 rows. Products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane holds
-// scores of one row only and the P that it computed is already the second product's operand: key slots are
-// permuted alike in P and V^T, which a sum over keys allows.
-template <class T, int D>
-__global__ __launch_bounds__(64 * kTileWaves) void attention_tile_kernel(const ls_hip_attention a, uint32_t page_shift) {
-    constexpr int kStride = D + 8;   // halves of an LDS row; 16 bytes of padding turn the banks
-    __shared__ __align__(16) short lds_k[kTileKeys * kStride];
-    __shared__ __align__(16) short lds_v[kTileKeys * kStride];
+template <int D>
+struct Tile {
+    static constexpr int kHalves = 1;
+    static constexpr int kWaves = D == 256 ? 4 : 8;
+    static constexpr int kRows = 32 * kHalves * kWaves;
+    static constexpr int kKeys = D == 256 ? 32 : 64;
+    static constexpr int kChunks = D / 8;                     // 16-byte chunks of a row
+    static constexpr int kLoads = kKeys * kChunks / (64 * kWaves);   // a wave's loads of a tile, 64 chunks each
+    static constexpr int kLoadRows = 64 / kChunks;            // rows of one load
+    // Chunk c of row r lies at position c ^ turn(r), so that 8 rows' chunks (K operands) and 4 rows' pairs of
+    // chunks (transposing reads) lie in different banks.
+    static constexpr int kTurn8 = 1;   // turn(r + 8) = turn(r) ^ 1 for r % 16 < 8
+    static __device__ __forceinline__ int turn(int r) {
+        return D == 64 ? (r >> 1 & 3) << 1 | (r >> 3 & 1) : (r & 7) << 1 | (r >> 3 & 1);
+    }
+};
+
+typedef __attribute__((address_space(3))) void* lds_void;
+typedef __attribute__((address_space(3))) char* lds_bytes;
+typedef const __attribute__((address_space(1))) void* global_void;
+
+template <class T, int D, bool Large>
+__global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(const ls_hip_attention a, uint32_t shift) {
+    typedef Tile<D> C;
+    constexpr int kHalves = C::kHalves, kKeys = C::kKeys, kSub = kKeys / 32;
+    __shared__ __align__(1024) short lds_k[2][kKeys * D];
+    __shared__ __align__(1024) short lds_v[2][kKeys * D];
 
     const int head = blockIdx.x % a.kv_heads;
     const int group = a.q_heads / a.kv_heads;
-    const int tile = blockIdx.x / a.kv_heads;
+    // the last tiles of a sequence see the most keys: they go first
+    const int tile = gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads;
     const Sequence seq = read_sequence(a, blockIdx.y);
     const int rows = seq.tokens * group;
-    const int row0 = tile * kTileRows;
+    const int row0 = tile * C::kRows;
     if (rows <= kShortRows || row0 >= rows) return;
-    const int row_end = min(row0 + kTileRows, rows);
+    const int row_end = min(row0 + C::kRows, rows);
     const int base = seq.keys - seq.tokens;   // position of token 0
     const int p_low = base + row0 / group, p_high = base + (row_end - 1) / group;
     const int window = (int)a.window, sinks = (int)a.sinks;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
-    const int row = min(row0 + 32 * wave + col, row_end - 1);
-    const bool store = row0 + 32 * wave + col < row_end;
-    const int token = row / group, q_head = head * group + row % group;
-    const int pos = base + token;
+    const int wave_row = row0 + 32 * kHalves * wave;
+    // positions of the wave's rows: what all of them see needs no masks
+    const int wave_low = base + min(wave_row, row_end - 1) / group;
+    const int wave_high = base + min(wave_row + 32 * kHalves - 1, row_end - 1) / group;
 
-    s16x8 q[D / 16];
-    {
-        const short* p = (const short*)a.q + (seq.first + token) * a.q_token_stride + q_head * a.q_head_stride + 8 * h;
+    int pos[kHalves];
+    s16x8 q[kHalves][D / 16];
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) q[i] = *(const s16x8*)(p + 16 * i);
+    for (int n = 0; n < kHalves; ++n) {
+        const int row = min(wave_row + 32 * n + col, row_end - 1), token = row / group;
+        pos[n] = base + token;
+        const short* p = (const short*)a.q + (seq.first + token) * a.q_token_stride +
+                         (head * group + row % group) * a.q_head_stride + 8 * h;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) q[n][i] = *(const s16x8*)(p + 16 * i);
     }
-    f32x16 o[D / 32] = {};
-    float m = kNoKey, l = 0.0f;
+    const Steps steps(kKeys, p_low, p_high, window, sinks);
+    const Table table = (Table)(a.page_table + blockIdx.y * a.table_stride);
     const float scale = a.scale * kLog2e;
 
-    const Steps steps(kTileKeys, p_low, p_high, window, sinks);
-    const int low = steps.low;
-
-    for (int t = 0; t < steps.count; ++t) {
+    // Loads of a tile: load i of a wave brings the rows 16-row block by block, row kLoadRows (wave + 4 i) + lane /
+    // kChunks. With pages of 16 keys and more, such a load lies in one page.
+    const int load_row = lane / C::kChunks;
+    const int last_page = (int)a.table_width - 1;
+    struct Pages {
+        int of[C::kLoads];
+    };
+    auto fetch = [&](int t) __attribute__((always_inline)) {
+        Pages pages;
         const int key0 = steps.key(t);
-        __syncthreads();   // every wave is done with the previous tile
-        for (int i = threadIdx.x; i < kTileKeys * (D / 8); i += 64 * kTileWaves) {
-            const int r = i / (D / 8), c = i % (D / 8), key = key0 + r;
-            s16x8 k = {}, v = {};
-            if (key <= p_high && (window == 0 || key >= low || key < sinks)) {
-                const int page = a.page_table[blockIdx.y * a.table_stride + (key >> page_shift)];
-                const int slot = key & ((1 << page_shift) - 1);
-                if ((uint32_t)page < a.pages) {
-                    k = *(const s16x8*)((const short*)a.k_pages + page * a.k_page_stride + head * a.k_head_stride +
-                                        slot * a.k_slot_stride + 8 * c);
-                    v = *(const s16x8*)((const short*)a.v_pages + page * a.v_page_stride + head * a.v_head_stride +
-                                        slot * a.v_slot_stride + 8 * c);
-                } else if (a.status) {
-                    atomicOr(a.status, (uint32_t)LS_STATUS_BAD_DESCRIPTOR);
-                }
-            }
-            *(s16x8*)(lds_k + r * kStride + 8 * c) = k;
-            *(s16x8*)(lds_v + r * kStride + 8 * c) = v;
+#pragma unroll
+        for (int i = 0; i < C::kLoads; ++i) {
+            const int r0 = C::kLoadRows * (wave + C::kWaves * i);
+            pages.of[i] = table[min((key0 + r0 + (Large ? 0 : load_row)) >> (int)shift, last_page)];
         }
+        return pages;
+    };
+    // A page that is none (or lies outside the cache): nobody's, or reported, and made zeros once it is here.
+    auto load = [&](const void* base, int64_t page_stride, int64_t head_stride, int64_t slot_stride, short* lds, int t,
+                    const Pages& pages) __attribute__((always_inline)) {
+        uint32_t bad = 0;
+        const int key0 = steps.key(t);
+#pragma unroll
+        for (int i = 0; i < C::kLoads; ++i) {
+            const int r0 = C::kLoadRows * (wave + C::kWaves * i), r = r0 + load_row;
+            int page = pages.of[i];
+            if ((uint32_t)page >= a.pages) page = 0, bad |= 1u << i;
+            const int slot = (key0 + (Large ? r0 : r)) & ((1 << shift) - 1);
+            const short* src = (const short*)base + page * page_stride + head * head_stride + slot * slot_stride;
+            uint32_t at = 8 * ((lane % C::kChunks) ^ C::turn(r));
+            if constexpr (Large) at += (uint32_t)(load_row * (int)slot_stride);
+            __builtin_amdgcn_global_load_lds((global_void)(src + at), (lds_void)(lds + r0 * D), 16, 0, 0);
+        }
+        return bad;
+    };
+    auto clear = [&](uint32_t bad, short* lds, int key0) {
+#pragma unroll
+        for (int i = 0; i < C::kLoads; ++i) {
+            if (!(bad >> i & 1)) continue;
+            const int r = C::kLoadRows * (wave + C::kWaves * i) + load_row, key = key0 + r;
+            *(s16x8*)(lds + r * D + 8 * (lane % C::kChunks)) = s16x8{};
+            if (key <= p_high && (window == 0 || key >= steps.low || key < sinks) && a.status)
+                atomicOr(a.status, (uint32_t)LS_STATUS_BAD_DESCRIPTOR);
+        }
+    };
+    auto load_k = [&](int t, const Pages& pages) __attribute__((always_inline)) {
+        return load(a.k_pages, a.k_page_stride, a.k_head_stride, a.k_slot_stride, lds_k[t & 1], t, pages);
+    };
+    auto load_v = [&](int t, const Pages& pages) __attribute__((always_inline)) {
+        return load(a.v_pages, a.v_page_stride, a.v_head_stride, a.v_slot_stride, lds_v[t & 1], t, pages);
+    };
+    // A lane's addresses in LDS. Rows are 2 D bytes, so the turned chunk index is a xor on the bits below them;
+    // what is left of an address is a constant of the instruction.
+    const uint32_t k_at = 2 * D * col + 16 * (h ^ C::turn(col));
+    const int v_row = 4 * h + (lane & 15) / 4;
+    const uint32_t v_at = 2 * D * v_row + 16 * ((2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ C::turn(v_row)) + 8 * (lane & 1);
+    // scores of a tile: register i of a lane is key 8 (i / 4) + 4 h + i % 4 of 32
+    auto keys = [&](const lds_bytes lds, int i, s16x8 (&k)[kSub]) {
+        const lds_bytes at = lds + (k_at ^ (32 * i));
+#pragma unroll
+        for (int kt = 0; kt < kSub; ++kt) k[kt] = *(__attribute__((address_space(3))) s16x8*)(at + 2 * D * 32 * kt);
+    };
+    // Scores of a tile, work(i) going on beside step i: the matrix cores take 32 cycles for a product that is issued
+    // in 4, and the operands of the next step are read meanwhile. The barriers keep the compiler from reading
+    // everything at once, which does not fit the registers.
+    auto scores = [&](f32x16 (&s)[kHalves][kSub], int t, auto work) __attribute__((always_inline)) {
+        const lds_bytes lds = (lds_bytes)lds_k + (t & 1) * (2 * D * kKeys);
+        s16x8 k[2][kSub];
+#pragma unroll
+        for (int kt = 0; kt < kSub; ++kt)
+#pragma unroll
+            for (int n = 0; n < kHalves; ++n) s[n][kt] = f32x16{};
+        keys(lds, 0, k[0]);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            if (i + 1 < D / 16) keys(lds, i + 1, k[(i + 1) & 1]);
+#pragma unroll
+            for (int kt = 0; kt < kSub; ++kt)
+#pragma unroll
+                for (int n = 0; n < kHalves; ++n) s[n][kt] = T::mfma32(k[i & 1][kt], q[n][i], s[n][kt]);
+            work(i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    // V^T operands: key slot (h, j) of step t16 is key 16 t16 + 8 (j / 4) + 4 h + j % 4
+    auto values = [&](int t, int t16, int d) __attribute__((always_inline)) {
+        const lds_bytes lds = (lds_bytes)lds_v + (t & 1) * (2 * D * kKeys);
+        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (v_at ^ (64 * d)) + 2 * D * 16 * t16));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_ptr)(lds + (v_at ^ (64 * d) ^ (16 * C::kTurn8)) + 2 * D * (16 * t16 + 8)));
+        return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto odd_values = [&](int t) __attribute__((always_inline)) {
+        bool odd = false;
+        for (int i = lane; i < kKeys * D / 8; i += 64) odd |= not_finite<T>(*(const s16x8*)(lds_v[t & 1] + 8 * i));
+        return __any(odd) != 0;
+    };
+    f32x16 o[kHalves][D / 32] = {};
+    float m[kHalves], l[kHalves];
+#pragma unroll
+    for (int n = 0; n < kHalves; ++n) m[n] = kNoKey, l[n] = 0.0f;
+
+    auto sees_all = [&](int key0, int low, int high) {   // rows from position low to high see every key of a tile
+        return key0 + kKeys - 1 <= low && (window == 0 || key0 > high - window || key0 + kKeys <= sinks);
+    };
+    auto mask = [&](f32x16 (&s)[kHalves][kSub], int key0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < kHalves; ++n)
+#pragma unroll
+            for (int kt = 0; kt < kSub; ++kt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!sees(key0 + 32 * kt + 8 * (i / 4) + 4 * h + i % 4, pos[n], window, sinks)) s[n][kt][i] = -INFINITY;
+    };
+    auto largest = [&](const f32x16 (&s)[kSub]) {
+        float top = kNoKey;
+#pragma unroll
+        for (int kt = 0; kt < kSub; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kt][i]);
+        return top;
+    };
+
+    bool later = false;
+    if (steps.count) {
+        f32x16 s[kHalves][kSub];
+        float top[kHalves];
+        // pages of the tiles t + 1 and t + 2
+        Pages pages1 = fetch(0), pages2 = fetch(1);
+        uint32_t bad_k = load_k(0, pages1), bad_v = load_v(0, pages1);
+        __builtin_amdgcn_s_waitcnt(0);
+        if (bad_k) clear(bad_k, lds_k[0], steps.key(0));
         __syncthreads();
-        const bool full = key0 + kTileKeys - 1 <= p_low &&
-                          (window == 0 || key0 > p_high - window || key0 + kTileKeys <= sinks);
+        bad_k = steps.count > 1 ? load_k(1, pages2) : 0;
+        pages1 = pages2;
+        pages2 = fetch(2);
+        scores(s, 0, [](int) {});
+#pragma unroll
+        for (int n = 0; n < kHalves; ++n) top[n] = largest(s[n]);
+        for (int t = 0; t < steps.count; ++t) {
+            const int key0 = steps.key(t);
+            const bool full = sees_all(key0, wave_low, wave_high);
+            // tile t of V and tile t + 1 of K are here, and every wave is done with the buffers before them
+            __builtin_amdgcn_s_waitcnt(0);
+            if (bad_v) clear(bad_v, lds_v[t & 1], key0);
+            if (bad_k) clear(bad_k, lds_k[(t + 1) & 1], steps.key(t + 1));
+            __syncthreads();
+            bad_v = t + 1 < steps.count ? load_v(t + 1, pages1) : 0;
+            bad_k = t + 2 < steps.count ? load_k(t + 2, pages2) : 0;
+            pages1 = pages2;
+            pages2 = fetch(t + 3);
 
-        // scores of 2 x 32 keys: register i of a lane is key 8 (i / 4) + 4 h + i % 4 of its 32
-        f32x16 s[2] = {};
+            // An infinity or NaN in a value must reach only the rows that see its key, and 0 * NaN is NaN: where not every
+            // row of the workgroup sees all keys, such values count as 0 here and are added to the result at the end.
+            if (!sees_all(key0, p_low, p_high) && odd_values(t)) {
+                later = true;
+                __syncthreads();
+                for (int i = threadIdx.x; i < kKeys * D / 8; i += 64 * C::kWaves) {
+                    s16x8 v = *(const s16x8*)(lds_v[t & 1] + 8 * i);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-                s[kt] = T::mfma32(*(const s16x8*)(lds_k + (32 * kt + col) * kStride + 16 * i + 8 * h), q[i], s[kt]);
-        float top = m;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float x = s[kt][i] * scale;
-                if (!full && !sees(key0 + 32 * kt + 8 * (i / 4) + 4 * h + i % 4, pos, window, sinks)) x = -INFINITY;
-                s[kt][i] = x;
-                top = fmaxf(top, x);
-            }
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float keep = __builtin_amdgcn_exp2f(m - top);
-        m = top;
-        float sum = 0.0f;
-        // P is rounded to the values' type for the matrix product; the sum takes it in fp32
-        u32x4 p[4];
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float x = __builtin_amdgcn_exp2f(s[kt][i] - m), y = __builtin_amdgcn_exp2f(s[kt][i + 1] - m);
-                sum += x + y;
-                p[2 * kt + i / 8][i % 8 / 2] = T::pack(x, y);
-            }
-        l = l * keep + sum;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) o[d] *= keep;
-
-        // key slot (h, j) of product step t: key 16 t + 8 (j / 4) + 4 h + j % 4
-        const int tr_row = 4 * h + (lane & 15) / 4, tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-#pragma unroll
-        for (int t16 = 0; t16 < 4; ++t16)
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                const short* at = lds_v + (16 * t16 + tr_row) * kStride + 32 * d + tr_col;
-                typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-                const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at));
-                const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 8 * kStride));
-                const s16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                if (!full) {
-                    // An infinity or NaN in a value must reach only the rows that see its key, and 0 * NaN is
-                    // NaN: such (rare) fragments are taken key by key, each added where it is seen.
-                    if (__ballot(not_finite<T>(v))) {
-                        const s16x8 pp = __builtin_bit_cast(s16x8, p[t16]);
-                        for (int slot = 0; slot < 16; ++slot) {
-                            s16x8 va = {}, pa = {};
-                            if (h == slot / 8) {
-#pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    if (j == slot % 8) va[j] = v[j], pa[j] = pp[j];
-                            }
-                            const f32x16 one = T::mfma32(va, pa, f32x16{});
-                            if (sees(key0 + 16 * t16 + 8 * (slot % 8 / 4) + 4 * (slot / 8) + slot % 4, pos, window, sinks))
-                                o[d] += one;
-                        }
-                        continue;
-                    }
+                    for (int j = 0; j < 8; ++j)
+                        if (((uint32_t)v[j] & T::kExponent) == T::kExponent) v[j] = 0;
+                    *(s16x8*)(lds_v[t & 1] + 8 * i) = v;
                 }
-                o[d] = T::mfma32(v, __builtin_bit_cast(s16x8, p[t16]), o[d]);
+                __syncthreads();
             }
+            if (!full) {
+                mask(s, key0);
+#pragma unroll
+                for (int n = 0; n < kHalves; ++n) top[n] = largest(s[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < kHalves; ++n) {
+                top[n] = fmaxf(top[n], __shfl_xor(top[n], 32)) * scale;
+                if (__any(top[n] > m[n] + kSlack)) {
+                    const float next_m = fmaxf(m[n], top[n]), keep = __builtin_amdgcn_exp2f(m[n] - next_m);
+                    m[n] = next_m;
+                    l[n] *= keep;
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d) o[n][d] *= keep;
+                }
+            }
+            // The next tile's scores (after the last one: of what the buffer held before, unused), and this one's P
+            // beside them: rounded to the values' type for the matrix product, summed in fp32.
+            f32x16 next[kHalves][kSub];
+            u32x4 p[kHalves][kKeys / 16];
+            scores(next, t + 1, [&](int step) __attribute__((always_inline)) {
+                constexpr int kPairs = kKeys / 4, kSteps = D / 16;
+#pragma unroll
+                for (int n = 0; n < kHalves; ++n)
+#pragma unroll
+                    for (int pair = step * kPairs / kSteps; pair < (step + 1) * kPairs / kSteps; ++pair) {
+                        const int kt = pair / 8, i = pair % 8 * 2;
+                        const float x = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i], scale, -m[n]));
+                        const float y = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i + 1], scale, -m[n]));
+                        l[n] += x + y;
+                        p[n][pair / 4][pair % 4] = T::pack(x, y);
+                    }
+            });
+#pragma unroll
+            for (int n = 0; n < kHalves; ++n) top[n] = kNoKey;
+            {
+                s16x8 v[2][D / 32];
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) v[0][d] = values(t, 0, d);
+#pragma unroll
+                for (int t16 = 0; t16 < kKeys / 16; ++t16) {
+                    if (t16 + 1 < kKeys / 16)
+#pragma unroll
+                        for (int d = 0; d < D / 32; ++d) v[(t16 + 1) & 1][d] = values(t, t16 + 1, d);
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                        for (int n = 0; n < kHalves; ++n)
+                            o[n][d] = T::mfma32(v[t16 & 1][d], __builtin_bit_cast(s16x8, p[n][t16]), o[n][d]);
+#pragma unroll
+                    for (int n = 0; n < kHalves; ++n)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) top[n] = fmaxf(top[n], next[n][t16 / 2][t16 % 2 * 8 + i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < kHalves; ++n) {
+#pragma unroll
+                for (int kt = 0; kt < kSub; ++kt) s[n][kt] = next[n][kt];
+            }
+        }
     }
-    l += __shfl_xor(l, 32);
-    if (!store) return;
-    const float inv = l > 0.0f ? 1.0f / l : l;   // NaN stays NaN
-    short* out = (short*)a.out + (seq.first + token) * a.out_token_stride + q_head * a.out_head_stride + 4 * h;
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+    for (int n = 0; n < kHalves; ++n) {
+        l[n] += __shfl_xor(l[n], 32);
+        const int row = wave_row + 32 * n + col;
+        if (row >= row_end) continue;
+        const int token = row / group, q_head = head * group + row % group;
+        const float inv = l[n] > 0.0f ? 1.0f / l[n] : l[n];   // NaN stays NaN
+        short* out = (short*)a.out + (seq.first + token) * a.out_token_stride + q_head * a.out_head_stride + 4 * h;
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-            *(u32x2*)(out + 32 * d + 2 * i) =
-                u32x2{T::pack(o[d][i] * inv, o[d][i + 1] * inv), T::pack(o[d][i + 2] * inv, o[d][i + 3] * inv)};
-    if (a.lse && h == 0)
-        a.lse[(int64_t)(seq.first + token) * a.q_heads + q_head] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *(u32x2*)(out + 32 * d + 2 * i) = u32x2{T::pack(o[n][d][i] * inv, o[n][d][i + 1] * inv),
+                                                       T::pack(o[n][d][i + 2] * inv, o[n][d][i + 3] * inv)};
+        if (a.lse && h == 0)
+            a.lse[(int64_t)(seq.first + token) * a.q_heads + q_head] = l[n] == 0.0f ? -INFINITY : m[n] * kLn2 + logf(l[n]);
+    }
+    // The values that counted as 0, where not all rows see a tile: their sum takes the place of what sees one.
+    if (!later) return;
+    __syncthreads();   // the results are stored
+    for (int i = threadIdx.x; i < (row_end - row0) * D; i += 64 * C::kWaves) {
+        const int row = row0 + i / D, c = i % D, token = row / group, q_head = head * group + row % group;
+        float sum = 0.0f;
+        for (int t = 0; t < steps.count; ++t) {
+            const int key0 = steps.key(t);
+            if (sees_all(key0, p_low, p_high)) continue;
+            for (int key = key0; key < key0 + kKeys; ++key) {
+                if (!sees(key, base + token, window, sinks)) continue;
+                const int page = a.page_table[blockIdx.y * a.table_stride + min(key >> (int)shift, last_page)];
+                if ((uint32_t)page >= a.pages) continue;
+                const short v = ((const short*)a.v_pages)[page * a.v_page_stride + head * a.v_head_stride +
+                                                         (key & ((1 << shift) - 1)) * a.v_slot_stride + c];
+                if (((uint32_t)v & T::kExponent) == T::kExponent) sum += T::to_float(v);
+            }
+        }
+        if (sum != 0.0f)
+            ((short*)a.out)[(seq.first + token) * a.out_token_stride + q_head * a.out_head_stride + c] = (short)T::pack(sum, 0.0f);
+    }
 }
 
 bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
@@ -608,8 +811,9 @@ void launch(const ls_hip_attention& a, hipStream_t stream) {
         else attention_rows_kernel<T, D, false><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan);
     }
     if (rows > (uint32_t)kShortRows) {
-        const dim3 grid((rows + kTileRows - 1) / kTileRows * a.kv_heads, a.sequences);
-        attention_tile_kernel<T, D><<<grid, 64 * kTileWaves, 0, stream>>>(a, shift);
+        const dim3 grid((rows + Tile<D>::kRows - 1) / Tile<D>::kRows * a.kv_heads, a.sequences);
+        if (a.page_size >= 16) attention_tile_kernel<T, D, true><<<grid, 64 * Tile<D>::kWaves, 0, stream>>>(a, shift);
+        else attention_tile_kernel<T, D, false><<<grid, 64 * Tile<D>::kWaves, 0, stream>>>(a, shift);
     }
 }
 
