@@ -12,6 +12,9 @@
 #include <cmath>
 #include "leanstream_hip.h"
 
+// Closures over register arrays are inlined, or the arrays would lie in memory.
+#define LS_INLINE __attribute__((always_inline))
+
 namespace lsamd {
 namespace {
 
@@ -19,6 +22,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -124,7 +128,7 @@ struct Steps {
 };
 
 // ---------------------------------------------------------------------------------
-// Few rows: one sequence's new tokens times the heads of a group, 16 rows a workgroup
+// Few rows: one sequence's new tokens times the heads of a group
 // ---------------------------------------------------------------------------------
 // Bound by the bytes of the cache. Keys go 32 at a time from memory straight into matrix operands, with no
 // LDS: a lane of S^T = K Q^T (16 x 16 x 32) holds 16 bytes of one key, and of V a lane loads the same D / 16
@@ -132,15 +136,13 @@ struct Steps {
 // workgroup take the steps of its split in turn and are joined through LDS; the splits of a long sequence are
 // joined by the workgroup that finishes last, in their order.
 constexpr int kRowWaves = 4;
-constexpr int kRows = 16;
+constexpr int kRows = 16;          // sequences of up to this many rows go this way
 constexpr int kStepKeys = 32;
-constexpr int kShortRows = 64;     // sequences of up to this many rows go this way
 
 struct SplitPlan {
     uint32_t splits;       // of the longest sequence
     uint32_t chunk;        // steps of a split, a multiple of kRowWaves
-    uint32_t row_blocks;
-    uint32_t rows;         // of a row block in the workspace
+    uint32_t rows;         // of a split in the workspace
     uint64_t bytes;        // of the workspace
 };
 
@@ -202,11 +204,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
     const int head = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
     const int group = a.q_heads / a.kv_heads;
     const Sequence seq = read_sequence(a, blockIdx.y);
-    const int rows = seq.tokens * group, row0 = blockIdx.z * kRows;
-    if (rows > kShortRows || row0 >= rows) return;
-    const int row_count = min(kRows, rows - row0);
+    const int rows = seq.tokens * group;
+    if (rows > kRows || rows == 0) return;
     const int base = seq.keys - seq.tokens;
-    const int p_low = base + row0 / group, p_high = base + (row0 + row_count - 1) / group;
+    const int p_low = base, p_high = seq.keys - 1;
     const int window = (int)a.window, sinks = (int)a.sinks;
     const Steps steps(kStepKeys, p_low, p_high, window, sinks);
     const int splits = max(1, (steps.count + (int)plan.chunk - 1) / (int)plan.chunk);
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, g = lane >> 4;
-    const int row = row0 + min(i16, row_count - 1);
+    const int row = min(i16, rows - 1);
     const int pos = base + row / group;
 
     s16x8 q[D / 32];
@@ -343,10 +344,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
     __syncthreads();
 
     // columns pairwise: thread -> (row, dims 2 c, 2 c + 1)
-    const uint32_t pair = (blockIdx.y * a.kv_heads + head) * plan.row_blocks + blockIdx.z;
+    const uint32_t pair = blockIdx.y * a.kv_heads + head;
     const uint32_t stride = plan.rows * (D + 2);   // floats of a split: rows of sums, then m and l of every row
     float* space = (float*)((char*)a.workspace + kCounterBytes) + (uint64_t)pair * plan.splits * stride;
-    const int items = row_count * (D / 2);
+    const int items = rows * (D / 2);
     for (int i = threadIdx.x; i < items; i += 64 * kRowWaves) {
         const int r = i / (D / 2), c = 2 * (i % (D / 2));
         float top = lds_m[0][r];
@@ -365,7 +366,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
             store_agent(part + r * D + c, x, y);
             if (c == 0) store_agent(part + plan.rows * D + 2 * r, top, sum);
         } else {
-            const int token = seq.first + (row0 + r) / group, q_head = head * group + (row0 + r) % group;
+            const int token = seq.first + r / group, q_head = head * group + r % group;
             const float inv = sum > 0.0f ? 1.0f / sum : sum;   // NaN stays NaN
             *(uint32_t*)((short*)a.out + token * a.out_token_stride + q_head * a.out_head_stride + c) = T::pack(x * inv, y * inv);
             if (a.lse && c == 0)
@@ -387,7 +388,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
     }
     __syncthreads();
     if (lds_turn != (uint32_t)splits - 1) return;
-    for (int i = threadIdx.x; i < row_count * D; i += 64 * kRowWaves) {
+    for (int i = threadIdx.x; i < rows * D; i += 64 * kRowWaves) {
         const int r = i / D, c = i % D;
         float top = kNoKey, x = 0.0f, sum = 0.0f;
         for (int s = 0; s < splits; ++s) {
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
             sum = sum * old + load_agent(part + plan.rows * D + 2 * r + 1) * f;
             top = next;
         }
-        const int token = seq.first + (row0 + r) / group, q_head = head * group + (row0 + r) % group;
+        const int token = seq.first + r / group, q_head = head * group + r % group;
         const float inv = sum > 0.0f ? 1.0f / sum : sum;
         ((short*)a.out)[token * a.out_token_stride + q_head * a.out_head_stride + c] = (short)T::pack(x * inv, 0.0f);
         if (a.lse && c == 0)
@@ -410,33 +411,41 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
 // ---------------------------------------------------------------------------------
 // Many rows
 // ---------------------------------------------------------------------------------
-// One workgroup: 4 waves of 32 * Halves rows of one sequence and KV head against all keys they see, Keys at a
-// time through LDS. Products are taken transposed, S^T = K Q^T and O^T = V^T P^T (32 x 32 x 16), so that a lane
-// holds scores of one row only and the P that it computed is already the second product's operand: key slots are
-// permuted alike in P and V^T, which a sum over keys allows. V^T comes out of LDS by transposing reads.
+// One workgroup: 8 waves of 32 rows of one sequence and KV head against the keys that they see, 64 at a time through
+// LDS. Products are taken transposed, S^T = K Q^T and O^T = V^T P^T (32 x 32 x 16), so that a lane holds scores of
+// one row only and the P that it computed is already the second product's operand: key slots are permuted alike in P
+// and V^T, which a sum over keys allows. V^T comes out of LDS by transposing reads.
 //
-// Bound by the matrix cores, the exponentials close behind: the scores of the next tile are multiplied while
-// those of this one go through the softmax. Tiles come from memory without passing registers, two buffers each
-// of K and V, one barrier a tile.
-// The running maximum moves only where a score exceeds it by more than this (base 2): until then P is at most
-// 2^8 instead of 1, and the sums need no scaling.
-constexpr float kSlack = 8.0f;
-
+// Bound by the matrix cores, LDS reads and exponentials close behind: the scores of the next tile are multiplied
+// while those of this one go through the softmax. Tiles come from memory without passing registers, two buffers
+// each of K and V, one barrier a tile. 4096 tokens over 32768 keys, 32 / 8 heads of 128: 2.1 ms, 980 TFLOP/s
+// (64 rows a wave, 4 waves, one buffer less read: 3.3 ms, its 512 registers leave one wave a SIMD).
+//
+// Where tiles are few, their keys are split; the parts go to the workspace in fp32 and are joined in order by
+// attention_join_kernel.
 template <int D>
 struct Tile {
-    static constexpr int kHalves = 1;
-    static constexpr int kWaves = D == 256 ? 4 : 8;
-    static constexpr int kRows = 32 * kHalves * kWaves;
+    static constexpr int kWaves = D == 256 ? 4 : 8;           // D = 256: twice the registers a row
+    static constexpr int kRows = 32 * kWaves;
     static constexpr int kKeys = D == 256 ? 32 : 64;
     static constexpr int kChunks = D / 8;                     // 16-byte chunks of a row
     static constexpr int kLoads = kKeys * kChunks / (64 * kWaves);   // a wave's loads of a tile, 64 chunks each
     static constexpr int kLoadRows = 64 / kChunks;            // rows of one load
     // Chunk c of row r lies at position c ^ turn(r), so that 8 rows' chunks (K operands) and 4 rows' pairs of
-    // chunks (transposing reads) lie in different banks.
-    static constexpr int kTurn8 = 1;   // turn(r + 8) = turn(r) ^ 1 for r % 16 < 8
+    // chunks (transposing reads) lie in different banks. turn(r + 8) = turn(r) ^ 1 for r % 16 < 8.
     static __device__ __forceinline__ int turn(int r) {
         return D == 64 ? (r >> 1 & 3) << 1 | (r >> 3 & 1) : (r & 7) << 1 | (r >> 3 & 1);
     }
+};
+// The running maximum moves only where a score exceeds it by more than this (base 2): until then P is at most
+// 2^8 instead of 1, and the sums need no scaling.
+constexpr float kSlack = 8.0f;
+
+struct TilePlan {
+    uint32_t splits;       // of the tile that sees most keys
+    uint32_t chunk;        // steps of a split
+    uint64_t offset;       // of the parts in the workspace: [split][token][q head] rows of D sums, then their m and l
+    uint64_t bytes;
 };
 
 typedef __attribute__((address_space(3))) void* lds_void;
@@ -444,9 +453,10 @@ typedef __attribute__((address_space(3))) char* lds_bytes;
 typedef const __attribute__((address_space(1))) void* global_void;
 
 template <class T, int D, bool Large>
-__global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(const ls_hip_attention a, uint32_t shift) {
+__global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(const ls_hip_attention a, uint32_t shift,
+                                                                              const TilePlan plan) {
     typedef Tile<D> C;
-    constexpr int kHalves = C::kHalves, kKeys = C::kKeys, kSub = kKeys / 32;
+    constexpr int kKeys = C::kKeys, kSub = kKeys / 32;
     __shared__ __align__(1024) short lds_k[2][kKeys * D];
     __shared__ __align__(1024) short lds_v[2][kKeys * D];
 
@@ -457,42 +467,43 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
     const Sequence seq = read_sequence(a, blockIdx.y);
     const int rows = seq.tokens * group;
     const int row0 = tile * C::kRows;
-    if (rows <= kShortRows || row0 >= rows) return;
+    if (rows <= kRows || row0 >= rows) return;
     const int row_end = min(row0 + C::kRows, rows);
     const int base = seq.keys - seq.tokens;   // position of token 0
     const int p_low = base + row0 / group, p_high = base + (row_end - 1) / group;
     const int window = (int)a.window, sinks = (int)a.sinks;
+    const Steps steps(kKeys, p_low, p_high, window, sinks);
+    const int begin = blockIdx.z * plan.chunk, end = min(begin + (int)plan.chunk, steps.count);
+    if (blockIdx.z && begin >= end) return;
+    const bool whole = steps.count <= (int)plan.chunk;   // no other split of this tile
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
-    const int wave_row = row0 + 32 * kHalves * wave;
+    const int wave_row = row0 + 32 * wave;
+    const bool active = wave_row < row_end;   // else the wave loads its part of the tiles and no more
     // positions of the wave's rows: what all of them see needs no masks
     const int wave_low = base + min(wave_row, row_end - 1) / group;
-    const int wave_high = base + min(wave_row + 32 * kHalves - 1, row_end - 1) / group;
+    const int wave_high = base + min(wave_row + 31, row_end - 1) / group;
 
-    int pos[kHalves];
-    s16x8 q[kHalves][D / 16];
+    const int row = min(wave_row + col, row_end - 1), token = row / group, q_head = head * group + row % group;
+    const int pos = base + token;
+    s16x8 q[D / 16];
+    {
+        const short* p = (const short*)a.q + (seq.first + token) * a.q_token_stride + q_head * a.q_head_stride + 8 * h;
 #pragma unroll
-    for (int n = 0; n < kHalves; ++n) {
-        const int row = min(wave_row + 32 * n + col, row_end - 1), token = row / group;
-        pos[n] = base + token;
-        const short* p = (const short*)a.q + (seq.first + token) * a.q_token_stride +
-                         (head * group + row % group) * a.q_head_stride + 8 * h;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) q[n][i] = *(const s16x8*)(p + 16 * i);
+        for (int i = 0; i < D / 16; ++i) q[i] = *(const s16x8*)(p + 16 * i);
     }
-    const Steps steps(kKeys, p_low, p_high, window, sinks);
     const Table table = (Table)(a.page_table + blockIdx.y * a.table_stride);
     const float scale = a.scale * kLog2e;
 
-    // Loads of a tile: load i of a wave brings the rows 16-row block by block, row kLoadRows (wave + 4 i) + lane /
-    // kChunks. With pages of 16 keys and more, such a load lies in one page.
+    // Loads of a tile: load i of a wave brings the rows kLoadRows (wave + kWaves i) + lane / kChunks. With pages of 16
+    // keys and more, such a load lies in one page.
     const int load_row = lane / C::kChunks;
     const int last_page = (int)a.table_width - 1;
     struct Pages {
         int of[C::kLoads];
     };
-    auto fetch = [&](int t) __attribute__((always_inline)) {
+    auto fetch = [&](int t) LS_INLINE {
         Pages pages;
         const int key0 = steps.key(t);
 #pragma unroll
@@ -503,8 +514,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
         return pages;
     };
     // A page that is none (or lies outside the cache): nobody's, or reported, and made zeros once it is here.
-    auto load = [&](const void* base, int64_t page_stride, int64_t head_stride, int64_t slot_stride, short* lds, int t,
-                    const Pages& pages) __attribute__((always_inline)) {
+    auto load = [&](const void* pool, int64_t page_stride, int64_t head_stride, int64_t slot_stride, short* lds, int t,
+                    const Pages& pages) LS_INLINE {
         uint32_t bad = 0;
         const int key0 = steps.key(t);
 #pragma unroll
@@ -513,93 +524,67 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
             int page = pages.of[i];
             if ((uint32_t)page >= a.pages) page = 0, bad |= 1u << i;
             const int slot = (key0 + (Large ? r0 : r)) & ((1 << shift) - 1);
-            const short* src = (const short*)base + page * page_stride + head * head_stride + slot * slot_stride;
+            const short* src = (const short*)pool + page * page_stride + head * head_stride + slot * slot_stride;
             uint32_t at = 8 * ((lane % C::kChunks) ^ C::turn(r));
             if constexpr (Large) at += (uint32_t)(load_row * (int)slot_stride);
             __builtin_amdgcn_global_load_lds((global_void)(src + at), (lds_void)(lds + r0 * D), 16, 0, 0);
         }
         return bad;
     };
+    auto some_row_sees = [&](int key) { return key <= p_high && (window == 0 || key >= steps.low || key < sinks); };
     auto clear = [&](uint32_t bad, short* lds, int key0) {
 #pragma unroll
         for (int i = 0; i < C::kLoads; ++i) {
             if (!(bad >> i & 1)) continue;
-            const int r = C::kLoadRows * (wave + C::kWaves * i) + load_row, key = key0 + r;
+            const int r = C::kLoadRows * (wave + C::kWaves * i) + load_row;
             *(s16x8*)(lds + r * D + 8 * (lane % C::kChunks)) = s16x8{};
-            if (key <= p_high && (window == 0 || key >= steps.low || key < sinks) && a.status)
-                atomicOr(a.status, (uint32_t)LS_STATUS_BAD_DESCRIPTOR);
+            if (some_row_sees(key0 + r) && a.status) atomicOr(a.status, (uint32_t)LS_STATUS_BAD_DESCRIPTOR);
         }
     };
-    auto load_k = [&](int t, const Pages& pages) __attribute__((always_inline)) {
+    auto load_k = [&](int t, const Pages& pages) LS_INLINE {
         return load(a.k_pages, a.k_page_stride, a.k_head_stride, a.k_slot_stride, lds_k[t & 1], t, pages);
     };
-    auto load_v = [&](int t, const Pages& pages) __attribute__((always_inline)) {
+    auto load_v = [&](int t, const Pages& pages) LS_INLINE {
         return load(a.v_pages, a.v_page_stride, a.v_head_stride, a.v_slot_stride, lds_v[t & 1], t, pages);
     };
-    // A lane's addresses in LDS. Rows are 2 D bytes, so the turned chunk index is a xor on the bits below them;
-    // what is left of an address is a constant of the instruction.
+    // A lane's addresses in LDS. Rows are 2 D bytes, so the turned chunk index is a xor on the bits below them; what is
+    // left of an address is a constant of the instruction.
     const uint32_t k_at = 2 * D * col + 16 * (h ^ C::turn(col));
     const int v_row = 4 * h + (lane & 15) / 4;
     const uint32_t v_at = 2 * D * v_row + 16 * ((2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ C::turn(v_row)) + 8 * (lane & 1);
-    // scores of a tile: register i of a lane is key 8 (i / 4) + 4 h + i % 4 of 32
-    auto keys = [&](const lds_bytes lds, int i, s16x8 (&k)[kSub]) {
+    auto keys = [&](const lds_bytes lds, int i, s16x8 (&k)[kSub]) LS_INLINE {
         const lds_bytes at = lds + (k_at ^ (32 * i));
 #pragma unroll
         for (int kt = 0; kt < kSub; ++kt) k[kt] = *(__attribute__((address_space(3))) s16x8*)(at + 2 * D * 32 * kt);
     };
-    // Scores of a tile, work(i) going on beside step i: the matrix cores take 32 cycles for a product that is issued
-    // in 4, and the operands of the next step are read meanwhile. The barriers keep the compiler from reading
-    // everything at once, which does not fit the registers.
-    auto scores = [&](f32x16 (&s)[kHalves][kSub], int t, auto work) __attribute__((always_inline)) {
+    // Scores of a tile (register i of a lane is key 8 (i / 4) + 4 h + i % 4 of 32), work(i) going on beside step i: the
+    // matrix cores take 32 cycles for a product that is issued in 4, and the operands of the next step are read
+    // meanwhile. The barriers keep the compiler from reading everything at once, which does not fit the registers.
+    auto scores = [&](f32x16 (&s)[kSub], int t, auto work) LS_INLINE {
         const lds_bytes lds = (lds_bytes)lds_k + (t & 1) * (2 * D * kKeys);
         s16x8 k[2][kSub];
 #pragma unroll
-        for (int kt = 0; kt < kSub; ++kt)
-#pragma unroll
-            for (int n = 0; n < kHalves; ++n) s[n][kt] = f32x16{};
+        for (int kt = 0; kt < kSub; ++kt) s[kt] = f32x16{};
         keys(lds, 0, k[0]);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
             if (i + 1 < D / 16) keys(lds, i + 1, k[(i + 1) & 1]);
 #pragma unroll
-            for (int kt = 0; kt < kSub; ++kt)
-#pragma unroll
-                for (int n = 0; n < kHalves; ++n) s[n][kt] = T::mfma32(k[i & 1][kt], q[n][i], s[n][kt]);
+            for (int kt = 0; kt < kSub; ++kt) s[kt] = T::mfma32(k[i & 1][kt], q[i], s[kt]);
             work(i);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-
     // V^T operands: key slot (h, j) of step t16 is key 16 t16 + 8 (j / 4) + 4 h + j % 4
-    auto values = [&](int t, int t16, int d) __attribute__((always_inline)) {
+    auto values = [&](int t, int t16, int d) LS_INLINE {
         const lds_bytes lds = (lds_bytes)lds_v + (t & 1) * (2 * D * kKeys);
         typedef __attribute__((address_space(3))) s16x4* lds_ptr;
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (v_at ^ (64 * d)) + 2 * D * 16 * t16));
-        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_ptr)(lds + (v_at ^ (64 * d) ^ (16 * C::kTurn8)) + 2 * D * (16 * t16 + 8)));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (v_at ^ (64 * d) ^ 16) + 2 * D * (16 * t16 + 8)));
         return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    auto odd_values = [&](int t) __attribute__((always_inline)) {
-        bool odd = false;
-        for (int i = lane; i < kKeys * D / 8; i += 64) odd |= not_finite<T>(*(const s16x8*)(lds_v[t & 1] + 8 * i));
-        return __any(odd) != 0;
-    };
-    f32x16 o[kHalves][D / 32] = {};
-    float m[kHalves], l[kHalves];
-#pragma unroll
-    for (int n = 0; n < kHalves; ++n) m[n] = kNoKey, l[n] = 0.0f;
-
     auto sees_all = [&](int key0, int low, int high) {   // rows from position low to high see every key of a tile
         return key0 + kKeys - 1 <= low && (window == 0 || key0 > high - window || key0 + kKeys <= sinks);
-    };
-    auto mask = [&](f32x16 (&s)[kHalves][kSub], int key0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < kHalves; ++n)
-#pragma unroll
-            for (int kt = 0; kt < kSub; ++kt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!sees(key0 + 32 * kt + 8 * (i / 4) + 4 * h + i % 4, pos[n], window, sinks)) s[n][kt][i] = -INFINITY;
     };
     auto largest = [&](const f32x16 (&s)[kSub]) {
         float top = kNoKey;
@@ -609,24 +594,42 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kt][i]);
         return top;
     };
-
-    bool later = false;
-    if (steps.count) {
-        f32x16 s[kHalves][kSub];
-        float top[kHalves];
-        // pages of the tiles t + 1 and t + 2
-        Pages pages1 = fetch(0), pages2 = fetch(1);
-        uint32_t bad_k = load_k(0, pages1), bad_v = load_v(0, pages1);
-        __builtin_amdgcn_s_waitcnt(0);
-        if (bad_k) clear(bad_k, lds_k[0], steps.key(0));
+    // An infinity or NaN in a value must reach only the rows that see its key, and 0 * NaN is NaN: where not every row of
+    // the workgroup sees all keys of a tile, such values become 0. True if one of them belongs to a row that sees it:
+    // it is then added to the result at the end.
+    auto settle = [&](int t, int key0) {
+        bool odd = false, seen = false;
+        for (int i = lane; i < kKeys * D / 8; i += 64) odd |= not_finite<T>(*(const s16x8*)(lds_v[t & 1] + 8 * i));
+        if (!__any(odd)) return false;   // every wave looks at the whole tile: all or none go on
         __syncthreads();
-        bad_k = steps.count > 1 ? load_k(1, pages2) : 0;
-        pages1 = pages2;
-        pages2 = fetch(2);
-        scores(s, 0, [](int) {});
+        for (int i = threadIdx.x; i < kKeys * D / 8; i += 64 * C::kWaves) {
+            s16x8 v = *(const s16x8*)(lds_v[t & 1] + 8 * i);
+            if (!not_finite<T>(v)) continue;
+            seen |= some_row_sees(key0 + i / C::kChunks);
 #pragma unroll
-        for (int n = 0; n < kHalves; ++n) top[n] = largest(s[n]);
-        for (int t = 0; t < steps.count; ++t) {
+            for (int j = 0; j < 8; ++j)
+                if (((uint32_t)v[j] & T::kExponent) == T::kExponent) v[j] = 0;
+            *(s16x8*)(lds_v[t & 1] + 8 * i) = v;
+        }
+        return __syncthreads_or(seen) != 0;
+    };
+
+    f32x16 o[D / 32] = {};
+    float m = kNoKey, l = 0.0f;
+    bool later = false;
+    if (begin < end) {
+        f32x16 s[kSub];
+        Pages pages1 = fetch(begin), pages2 = fetch(begin + 1);   // of the tiles t + 1 and t + 2
+        uint32_t bad_k = load_k(begin, pages1), bad_v = load_v(begin, pages1);
+        __builtin_amdgcn_s_waitcnt(0);
+        if (bad_k) clear(bad_k, lds_k[begin & 1], steps.key(begin));
+        __syncthreads();
+        bad_k = begin + 1 < end ? load_k(begin + 1, pages2) : 0;
+        pages1 = pages2;
+        pages2 = fetch(begin + 2);
+        scores(s, begin, [](int) {});
+        float top = largest(s);
+        for (int t = begin; t < end; ++t) {
             const int key0 = steps.key(t);
             const bool full = sees_all(key0, wave_low, wave_high);
             // tile t of V and tile t + 1 of K are here, and every wave is done with the buffers before them
@@ -634,126 +637,151 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
             if (bad_v) clear(bad_v, lds_v[t & 1], key0);
             if (bad_k) clear(bad_k, lds_k[(t + 1) & 1], steps.key(t + 1));
             __syncthreads();
-            bad_v = t + 1 < steps.count ? load_v(t + 1, pages1) : 0;
-            bad_k = t + 2 < steps.count ? load_k(t + 2, pages2) : 0;
+            bad_v = t + 1 < end ? load_v(t + 1, pages1) : 0;
+            bad_k = t + 2 < end ? load_k(t + 2, pages2) : 0;
             pages1 = pages2;
             pages2 = fetch(t + 3);
+            if (!sees_all(key0, p_low, p_high)) later |= settle(t, key0);
+            if (!active) continue;
 
-            // An infinity or NaN in a value must reach only the rows that see its key, and 0 * NaN is NaN: where not every
-            // row of the workgroup sees all keys, such values count as 0 here and are added to the result at the end.
-            if (!sees_all(key0, p_low, p_high) && odd_values(t)) {
-                later = true;
-                __syncthreads();
-                for (int i = threadIdx.x; i < kKeys * D / 8; i += 64 * C::kWaves) {
-                    s16x8 v = *(const s16x8*)(lds_v[t & 1] + 8 * i);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (((uint32_t)v[j] & T::kExponent) == T::kExponent) v[j] = 0;
-                    *(s16x8*)(lds_v[t & 1] + 8 * i) = v;
-                }
-                __syncthreads();
-            }
             if (!full) {
-                mask(s, key0);
 #pragma unroll
-                for (int n = 0; n < kHalves; ++n) top[n] = largest(s[n]);
+                for (int kt = 0; kt < kSub; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!sees(key0 + 32 * kt + 8 * (i / 4) + 4 * h + i % 4, pos, window, sinks)) s[kt][i] = -INFINITY;
+                top = largest(s);
             }
+            top = fmaxf(top, __shfl_xor(top, 32)) * scale;
+            if (__any(top > m + kSlack)) {
+                const float next_m = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - next_m);
+                m = next_m;
+                l *= keep;
 #pragma unroll
-            for (int n = 0; n < kHalves; ++n) {
-                top[n] = fmaxf(top[n], __shfl_xor(top[n], 32)) * scale;
-                if (__any(top[n] > m[n] + kSlack)) {
-                    const float next_m = fmaxf(m[n], top[n]), keep = __builtin_amdgcn_exp2f(m[n] - next_m);
-                    m[n] = next_m;
-                    l[n] *= keep;
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d) o[n][d] *= keep;
-                }
+                for (int d = 0; d < D / 32; ++d) o[d] *= keep;
             }
-            // The next tile's scores (after the last one: of what the buffer held before, unused), and this one's P
-            // beside them: rounded to the values' type for the matrix product, summed in fp32.
-            f32x16 next[kHalves][kSub];
-            u32x4 p[kHalves][kKeys / 16];
-            scores(next, t + 1, [&](int step) __attribute__((always_inline)) {
+            // The next tile's scores (after the last one: of what the buffer held before, unused), and this one's P beside
+            // them: rounded to the values' type for the matrix product, summed in fp32.
+            f32x16 next[kSub];
+            u32x4 p[kKeys / 16];
+            scores(next, t + 1, [&](int step) LS_INLINE {
                 constexpr int kPairs = kKeys / 4, kSteps = D / 16;
 #pragma unroll
-                for (int n = 0; n < kHalves; ++n)
-#pragma unroll
-                    for (int pair = step * kPairs / kSteps; pair < (step + 1) * kPairs / kSteps; ++pair) {
-                        const int kt = pair / 8, i = pair % 8 * 2;
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i], scale, -m[n]));
-                        const float y = __builtin_amdgcn_exp2f(fmaf(s[n][kt][i + 1], scale, -m[n]));
-                        l[n] += x + y;
-                        p[n][pair / 4][pair % 4] = T::pack(x, y);
-                    }
-            });
-#pragma unroll
-            for (int n = 0; n < kHalves; ++n) top[n] = kNoKey;
-            {
-                s16x8 v[2][D / 32];
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d) v[0][d] = values(t, 0, d);
-#pragma unroll
-                for (int t16 = 0; t16 < kKeys / 16; ++t16) {
-                    if (t16 + 1 < kKeys / 16)
-#pragma unroll
-                        for (int d = 0; d < D / 32; ++d) v[(t16 + 1) & 1][d] = values(t, t16 + 1, d);
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                        for (int n = 0; n < kHalves; ++n)
-                            o[n][d] = T::mfma32(v[t16 & 1][d], __builtin_bit_cast(s16x8, p[n][t16]), o[n][d]);
-#pragma unroll
-                    for (int n = 0; n < kHalves; ++n)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) top[n] = fmaxf(top[n], next[n][t16 / 2][t16 % 2 * 8 + i]);
-                    __builtin_amdgcn_sched_barrier(0);
+                for (int pair = step * kPairs / kSteps; pair < (step + 1) * kPairs / kSteps; ++pair) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[pair / 8][pair % 8 * 2], scale, -m));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(s[pair / 8][pair % 8 * 2 + 1], scale, -m));
+                    l += x + y;
+                    p[pair / 4][pair % 4] = T::pack(x, y);
                 }
+            });
+            // the second product, and the next tile's largest scores beside it
+            top = kNoKey;
+            s16x8 v[2][D / 32];
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) v[0][d] = values(t, 0, d);
+#pragma unroll
+            for (int t16 = 0; t16 < kKeys / 16; ++t16) {
+                if (t16 + 1 < kKeys / 16)
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d) v[(t16 + 1) & 1][d] = values(t, t16 + 1, d);
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) o[d] = T::mfma32(v[t16 & 1][d], __builtin_bit_cast(s16x8, p[t16]), o[d]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, next[t16 / 2][t16 % 2 * 8 + i]);
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int n = 0; n < kHalves; ++n) {
-#pragma unroll
-                for (int kt = 0; kt < kSub; ++kt) s[n][kt] = next[n][kt];
-            }
+            for (int kt = 0; kt < kSub; ++kt) s[kt] = next[kt];
         }
     }
+    l += __shfl_xor(l, 32);
+    const int64_t at = (int64_t)(seq.first + token) * a.q_heads + q_head;
+    const int64_t part_rows = (int64_t)a.tokens * a.q_heads;
+    float* parts = (float*)((char*)a.workspace + plan.offset) + blockIdx.z * part_rows * (D + 2);
+    if (wave_row + col < row_end) {
+        if (whole) {
+            const float inv = l > 0.0f ? 1.0f / l : l;   // NaN stays NaN
+            short* out = (short*)a.out + (seq.first + token) * a.out_token_stride + q_head * a.out_head_stride + 4 * h;
 #pragma unroll
-    for (int n = 0; n < kHalves; ++n) {
-        l[n] += __shfl_xor(l[n], 32);
-        const int row = wave_row + 32 * n + col;
-        if (row >= row_end) continue;
-        const int token = row / group, q_head = head * group + row % group;
-        const float inv = l[n] > 0.0f ? 1.0f / l[n] : l[n];   // NaN stays NaN
-        short* out = (short*)a.out + (seq.first + token) * a.out_token_stride + q_head * a.out_head_stride + 4 * h;
+            for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
+                for (int i = 0; i < 16; i += 4)
+                    *(u32x2*)(out + 32 * d + 2 * i) =
+                        u32x2{T::pack(o[d][i] * inv, o[d][i + 1] * inv), T::pack(o[d][i + 2] * inv, o[d][i + 3] * inv)};
+            if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *(u32x2*)(out + 32 * d + 2 * i) = u32x2{T::pack(o[n][d][i] * inv, o[n][d][i + 1] * inv),
-                                                       T::pack(o[n][d][i + 2] * inv, o[n][d][i + 3] * inv)};
-        if (a.lse && h == 0)
-            a.lse[(int64_t)(seq.first + token) * a.q_heads + q_head] = l[n] == 0.0f ? -INFINITY : m[n] * kLn2 + logf(l[n]);
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *(f32x4*)(parts + at * D + 32 * d + 2 * i + 4 * h) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+            if (h == 0) *(f32x2*)(parts + part_rows * D + 2 * at) = f32x2{m, l};
+        }
     }
-    // The values that counted as 0, where not all rows see a tile: their sum takes the place of what sees one.
+    // The values that became 0: their sum takes the place of the result of every row that sees one.
     if (!later) return;
     __syncthreads();   // the results are stored
     for (int i = threadIdx.x; i < (row_end - row0) * D; i += 64 * C::kWaves) {
-        const int row = row0 + i / D, c = i % D, token = row / group, q_head = head * group + row % group;
+        const int r = row0 + i / D, c = i % D, its = r / group, its_head = head * group + r % group;
         float sum = 0.0f;
-        for (int t = 0; t < steps.count; ++t) {
+        for (int t = begin; t < end; ++t) {
             const int key0 = steps.key(t);
             if (sees_all(key0, p_low, p_high)) continue;
             for (int key = key0; key < key0 + kKeys; ++key) {
-                if (!sees(key, base + token, window, sinks)) continue;
-                const int page = a.page_table[blockIdx.y * a.table_stride + min(key >> (int)shift, last_page)];
+                if (!sees(key, base + its, window, sinks)) continue;
+                const int page = table[min(key >> (int)shift, last_page)];
                 if ((uint32_t)page >= a.pages) continue;
                 const short v = ((const short*)a.v_pages)[page * a.v_page_stride + head * a.v_head_stride +
                                                          (key & ((1 << shift) - 1)) * a.v_slot_stride + c];
                 if (((uint32_t)v & T::kExponent) == T::kExponent) sum += T::to_float(v);
             }
         }
-        if (sum != 0.0f)
-            ((short*)a.out)[(seq.first + token) * a.out_token_stride + q_head * a.out_head_stride + c] = (short)T::pack(sum, 0.0f);
+        if (sum == 0.0f) continue;
+        if (whole)
+            ((short*)a.out)[(seq.first + its) * a.out_token_stride + its_head * a.out_head_stride + c] = (short)T::pack(sum, 0.0f);
+        else parts[((int64_t)(seq.first + its) * a.q_heads + its_head) * D + c] = sum;
     }
+}
+
+// Joins the parts of split tiles, a wave a row, in the order of the splits.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attention_join_kernel(const ls_hip_attention a, const TilePlan plan) {
+    constexpr int kLane = D / 64;
+    typedef float lane_sums __attribute__((ext_vector_type(kLane)));
+    const int64_t at = blockIdx.x * 4ll + (threadIdx.x >> 6), part_rows = (int64_t)a.tokens * a.q_heads;
+    if (at >= part_rows) return;
+    const int lane = threadIdx.x & 63, t = (int)(at / a.q_heads), q_head = (int)(at % a.q_heads);
+    const int group = a.q_heads / a.kv_heads;
+    // the sequence of token t: the last one that starts at or before it
+    int s = 0;
+    for (int s0 = 0; s0 < (int)a.sequences; s0 += 64) {
+        const uint64_t before = __ballot(s0 + lane < (int)a.sequences && a.q_start[min(s0 + lane, (int)a.sequences - 1)] <= t);
+        if (!before) break;
+        s = s0 + 63 - __clzll((long long)before);
+    }
+    const Sequence seq = read_sequence(a, __builtin_amdgcn_readfirstlane(s));
+    const int rows = seq.tokens * group;
+    if (rows <= kRows || t < seq.first || t >= seq.first + seq.tokens) return;
+    const int row0 = ((t - seq.first) * group + q_head % group) / Tile<D>::kRows * Tile<D>::kRows;
+    const int row_end = min(row0 + Tile<D>::kRows, rows), base = seq.keys - seq.tokens;
+    const Steps steps(Tile<D>::kKeys, base + row0 / group, base + (row_end - 1) / group, (int)a.window, (int)a.sinks);
+    if (steps.count <= (int)plan.chunk) return;   // one split: the result is written
+    const float* parts = (const float*)((const char*)a.workspace + plan.offset);
+    lane_sums o = {};
+    float m = kNoKey, l = 0.0f;
+    for (int begin = 0; begin < steps.count; begin += plan.chunk, parts += part_rows * (D + 2)) {
+        const f32x2 ml = *(const f32x2*)(parts + part_rows * D + 2 * at);
+        const lane_sums x = *(const lane_sums*)(parts + at * D + kLane * lane);
+        const float next = fmaxf(m, ml[0]), old = __builtin_amdgcn_exp2f(m - next), f = __builtin_amdgcn_exp2f(ml[0] - next);
+        o = o * old + x * f;
+        l = l * old + ml[1] * f;
+        m = next;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : l;   // NaN stays NaN
+    short* out = (short*)a.out + (int64_t)t * a.out_token_stride + q_head * a.out_head_stride + kLane * lane;
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) out[i] = (short)T::pack(o[i] * inv, 0.0f);
+    if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
@@ -782,18 +810,19 @@ int check(const ls_hip_attention& a) {
     return 0;
 }
 
+// Steps of `unit` keys that rows of up to `span` neighbouring tokens see.
+uint64_t most_steps(const ls_hip_attention& a, uint64_t unit, uint64_t span) {
+    const uint64_t steps = (a.max_context + unit - 1) / unit;
+    if (!a.window) return steps;
+    return std::min(steps, (a.window + span + unit - 1) / unit + 1 + (a.sinks + unit - 1) / unit);
+}
+
 // Splits of the sequences that take the row kernel: enough workgroups to fill the card, none with less than a
 // step for each of its waves. Where there are kFill groups already, there is one split.
 SplitPlan plan_rows(const ls_hip_attention& a) {
-    const uint32_t rows = std::min<uint64_t>((uint64_t)a.max_new * (a.q_heads / a.kv_heads), kShortRows);
     SplitPlan p{};
-    p.row_blocks = (rows + kRows - 1) / kRows;
-    p.rows = std::min<uint32_t>(rows, kRows);
-    uint64_t steps = (a.max_context + kStepKeys - 1) / kStepKeys;
-    if (a.window)
-        steps = std::min<uint64_t>(steps, ((uint64_t)a.window + a.max_new + kStepKeys - 1) / kStepKeys + 1 +
-                                              (a.sinks + kStepKeys - 1) / kStepKeys);
-    const uint64_t groups = (uint64_t)a.sequences * a.kv_heads * p.row_blocks;
+    p.rows = (uint32_t)std::min<uint64_t>((uint64_t)a.max_new * (a.q_heads / a.kv_heads), kRows);
+    const uint64_t steps = most_steps(a, kStepKeys, kRows), groups = (uint64_t)a.sequences * a.kv_heads;
     const uint64_t chunk = std::max<uint64_t>(1, (steps * groups + kFill - 1) / kFill);
     p.chunk = (uint32_t)std::min<uint64_t>((chunk + kRowWaves - 1) / kRowWaves * kRowWaves, 1u << 30);
     p.splits = (uint32_t)std::max<uint64_t>(1, (steps + p.chunk - 1) / p.chunk);
@@ -801,27 +830,64 @@ SplitPlan plan_rows(const ls_hip_attention& a) {
     return p;
 }
 
+// Splits of the tiles: two workgroups a compute unit if the tokens at hand all belong to chunks, none with less than 8
+// steps (its part of the sums costs as much as one).
+TilePlan plan_tiles(const ls_hip_attention& a, uint32_t tile_rows, uint32_t tile_keys, uint64_t offset) {
+    TilePlan p{};
+    const uint64_t group = a.q_heads / a.kv_heads, rows = a.tokens * group;
+    const uint64_t tiles = rows / tile_rows + std::min<uint64_t>(a.sequences, rows / (kRows + 1) + 1);
+    const uint64_t steps = most_steps(a, tile_keys, tile_rows / group + 2);
+    const uint64_t splits = std::max<uint64_t>(1, 512 / (tiles * a.kv_heads));
+    p.chunk = (uint32_t)std::max<uint64_t>(8, (steps + splits - 1) / splits);
+    p.splits = (uint32_t)std::max<uint64_t>(1, (steps + p.chunk - 1) / p.chunk);
+    p.offset = (offset + 255) / 256 * 256;
+    if (p.splits > 1) p.bytes = p.offset + p.splits * (uint64_t)a.tokens * a.q_heads * (a.head_dim + 2) * sizeof(float);
+    return p;
+}
+
+struct Plan {
+    bool by_rows, by_tiles;
+    SplitPlan rows;
+    TilePlan tiles;
+    uint64_t bytes;
+};
+Plan make_plan(const ls_hip_attention& a) {
+    Plan p{};
+    const uint32_t group = a.q_heads / a.kv_heads;
+    p.by_rows = group <= (uint32_t)kRows;
+    p.by_tiles = (uint64_t)a.max_new * group > (uint64_t)kRows;
+    if (p.by_rows) p.rows = plan_rows(a);
+    if (p.by_tiles)
+        p.tiles = a.head_dim == 256 ? plan_tiles(a, Tile<256>::kRows, Tile<256>::kKeys, p.rows.bytes)
+                                    : plan_tiles(a, Tile<128>::kRows, Tile<128>::kKeys, p.rows.bytes);
+    p.bytes = std::max(p.rows.bytes, p.tiles.bytes);
+    return p;
+}
+
 template <class T, int D>
-void launch(const ls_hip_attention& a, hipStream_t stream) {
-    const uint32_t group = a.q_heads / a.kv_heads, rows = a.max_new * group, shift = __builtin_ctz(a.page_size);
-    if (group <= (uint32_t)kShortRows) {
-        const SplitPlan plan = plan_rows(a);
-        const dim3 grid(plan.splits * a.kv_heads, a.sequences, plan.row_blocks);
-        if (a.page_size >= 16) attention_rows_kernel<T, D, true><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan);
-        else attention_rows_kernel<T, D, false><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan);
+void launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
+    const uint32_t shift = __builtin_ctz(a.page_size);
+    if (plan.by_rows) {
+        const dim3 grid(plan.rows.splits * a.kv_heads, a.sequences);
+        if (a.page_size >= 16) attention_rows_kernel<T, D, true><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan.rows);
+        else attention_rows_kernel<T, D, false><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan.rows);
     }
-    if (rows > (uint32_t)kShortRows) {
-        const dim3 grid((rows + Tile<D>::kRows - 1) / Tile<D>::kRows * a.kv_heads, a.sequences);
-        if (a.page_size >= 16) attention_tile_kernel<T, D, true><<<grid, 64 * Tile<D>::kWaves, 0, stream>>>(a, shift);
-        else attention_tile_kernel<T, D, false><<<grid, 64 * Tile<D>::kWaves, 0, stream>>>(a, shift);
+    if (plan.by_tiles) {
+        typedef Tile<D> C;
+        const uint32_t rows = a.max_new * (a.q_heads / a.kv_heads);
+        const dim3 grid((rows + C::kRows - 1) / C::kRows * a.kv_heads, a.sequences, plan.tiles.splits);
+        if (a.page_size >= 16) attention_tile_kernel<T, D, true><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
+        else attention_tile_kernel<T, D, false><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
+        if (plan.tiles.splits > 1)
+            attention_join_kernel<T, D><<<(uint32_t)(((uint64_t)a.tokens * a.q_heads + 3) / 4), 256, 0, stream>>>(a, plan.tiles);
     }
 }
 
 template <class T>
-void launch(const ls_hip_attention& a, hipStream_t stream) {
-    if (a.head_dim == 64) launch<T, 64>(a, stream);
-    else if (a.head_dim == 128) launch<T, 128>(a, stream);
-    else launch<T, 256>(a, stream);
+void launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
+    if (a.head_dim == 64) launch<T, 64>(a, plan, stream);
+    else if (a.head_dim == 128) launch<T, 128>(a, plan, stream);
+    else launch<T, 256>(a, plan, stream);
 }
 
 }  // namespace
@@ -829,8 +895,8 @@ void launch(const ls_hip_attention& a, hipStream_t stream) {
 
 extern "C" uint64_t ls_hip_attention_workspace(const ls_hip_attention* a) {
     using namespace lsamd;
-    if (!a || check(*a) || !a->tokens || !a->max_new || a->q_heads / a->kv_heads > (uint32_t)kShortRows) return 0;
-    return plan_rows(*a).bytes;
+    if (!a || check(*a) || !a->tokens || !a->max_new) return 0;
+    return make_plan(*a).bytes;
 }
 
 extern "C" int ls_hip_attention_enqueue(const ls_hip_attention* a, void* stream) {
@@ -838,10 +904,10 @@ extern "C" int ls_hip_attention_enqueue(const ls_hip_attention* a, void* stream)
     if (!a) return EINVAL;
     if (const int rc = check(*a)) return rc;
     if (!a->tokens || !a->max_new) return 0;
-    const uint64_t need = ls_hip_attention_workspace(a);
-    if (need && (!a->workspace || a->workspace_bytes < need)) return ENOSPC;
-    if (a->dtype == LS_TYPE_F16) launch<F16>(*a, static_cast<hipStream_t>(stream));
-    else launch<BF16>(*a, static_cast<hipStream_t>(stream));
+    const Plan plan = make_plan(*a);
+    if (plan.bytes && (!a->workspace || a->workspace_bytes < plan.bytes)) return ENOSPC;
+    if (a->dtype == LS_TYPE_F16) launch<F16>(*a, plan, static_cast<hipStream_t>(stream));
+    else launch<BF16>(*a, plan, static_cast<hipStream_t>(stream));
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : static_cast<int>(e);
 }
