@@ -80,10 +80,11 @@ struct Sequence {
 };
 
 // A sequence's lengths, held against the block's bounds: what lies outside has no tokens (their place in
-// q is unknown) or no keys.
+// q is unknown) or no keys. Ints: a pointer to int32_t or a Table.
+template <class Ints>
 __device__ __forceinline__ Sequence read_sequence(const ls_hip_attention& a, int s) {
-    const int q0 = ((Table)a.q_start)[s], q1 = ((Table)a.q_start)[s + 1];
-    Sequence q{q0, q1 - q0, ((Table)a.context)[s]};
+    const int q0 = ((Ints)a.q_start)[s], q1 = ((Ints)a.q_start)[s + 1];
+    Sequence q{q0, q1 - q0, ((Ints)a.context)[s]};
     bool bad = false;
     if (q0 < 0 || q1 < q0 || q1 > (int)a.tokens || (uint32_t)(q1 - q0) > a.max_new) {
         q.tokens = 0;
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
 
     const int head = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads;
     const int group = a.q_heads / a.kv_heads;
-    const Sequence seq = read_sequence(a, blockIdx.y);
+    const Sequence seq = read_sequence<Table>(a, blockIdx.y);
     const int rows = seq.tokens * group;
     if (rows > kRows || rows == 0) return;
     const int base = seq.keys - seq.tokens;
@@ -442,10 +443,100 @@ struct Tile {
 constexpr float kSlack = 8.0f;
 
 struct TilePlan {
-    uint32_t splits;       // of the tile that sees most keys
-    uint32_t chunk;        // steps of a split
-    uint64_t offset;       // of the parts in the workspace: [split][token][q head] rows of D sums, then their m and l
+    uint32_t splits;       // of a tile, at most
+    uint64_t offset;       // in the workspace: the steps of a split, then from kPartsAt on the parts, [split][token][q head]
+                           // rows of D sums and then their m and l
     uint64_t bytes;
+};
+constexpr uint32_t kTileFill = 256;    // workgroups that run at once: one a compute unit
+constexpr uint64_t kPartsAt = 256;
+constexpr uint32_t kLeastChunk = 8;    // steps: a split's part of the sums costs as much as one
+
+// Steps of `unit` keys that rows of up to `span` neighbouring tokens of a sequence see, at most.
+__host__ __device__ inline uint64_t most_steps(uint64_t keys, uint64_t unit, uint64_t span, uint64_t window, uint64_t sinks) {
+    const uint64_t steps = (keys + unit - 1) / unit, some = (window + span + unit - 1) / unit + 1 + (sinks + unit - 1) / unit;
+    return window && some < steps ? some : steps;
+}
+
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+// The tiles of all sequences and their splits. Only the device knows the lengths, so every wave reads them, 64 sequences
+// at a time. `chunk`, the steps of a split, is the least that makes no more than kTileFill workgroups: a second round
+// for a few of them costs more than it shortens the first, and so do parts of sums for tiles that fill the card by
+// themselves (4096 tokens over 4096 keys, 16 heads of 64: 103 us whole, 143 us split into 512).
+template <int D>
+struct TileWork {
+    typedef Tile<D> C;
+    uint32_t chunk;
+    int seq, tile, split;   // of an item; seq -1: there is none
+    __device__ __forceinline__ static uint32_t tiles_of(const ls_hip_attention& a, int s, uint32_t* steps) {
+        const uint32_t group = a.q_heads / a.kv_heads;
+        *steps = 0;
+        if (s >= (int)a.sequences) return 0;
+        const Sequence q = read_sequence<const int32_t*>(a, s);
+        const uint32_t rows = q.tokens * group;
+        if (rows <= (uint32_t)kRows) return 0;
+        *steps = (uint32_t)most_steps(q.keys, C::kKeys, C::kRows / group + 2, a.window, a.sinks);
+        return (rows + C::kRows - 1) / C::kRows;
+    }
+    __device__ __forceinline__ TileWork(const ls_hip_attention& a, const TilePlan& plan) {
+        const int lane = threadIdx.x & 63;
+        uint32_t total = 0, longest = 0, tiles = 0, n, steps;
+        for (int s0 = 0; s0 < (int)a.sequences; s0 += 64) {
+            n = tiles_of(a, s0 + lane, &steps);
+            total += n * steps;
+            tiles += n;
+            longest = max(longest, steps);
+        }
+        tiles = wave_sum(tiles) * a.kv_heads;
+#pragma unroll
+        for (int d = 32; d; d >>= 1) longest = max(longest, (uint32_t)__shfl_xor(longest, d));
+        longest = __builtin_amdgcn_readfirstlane(longest);
+        chunk = max(longest, 1u);
+        if (plan.splits == 1 || 2 * tiles > kTileFill) return;
+        // fewer than 2^8 tiles of fewer than 2^24 steps
+        chunk = max(max((wave_sum(total) * a.kv_heads + kTileFill - 1) / kTileFill, (longest + plan.splits - 1) / plan.splits), kLeastChunk);
+        for (;;) {   // twice the even share makes at most kTileFill / 2 + tiles
+            uint32_t items = 0;
+            for (int s0 = 0; s0 < (int)a.sequences; s0 += 64) {
+                if (a.sequences > 64) n = tiles_of(a, s0 + lane, &steps);
+                items += n * ((steps + chunk - 1) / chunk);
+            }
+            if (wave_sum(items) * a.kv_heads <= kTileFill || chunk >= longest) break;
+            chunk += chunk / 8 + 1;
+        }
+    }
+    __device__ __forceinline__ void find(const ls_hip_attention& a, uint32_t item) {
+        const int lane = threadIdx.x & 63;
+        uint32_t before = 0;
+        seq = -1;
+        for (int s0 = 0; s0 < (int)a.sequences && seq < 0; s0 += 64) {
+            uint32_t steps;
+            const uint32_t tiles = tiles_of(a, s0 + lane, &steps);
+            const uint32_t splits = max(1u, (steps + chunk - 1) / chunk), items = tiles * splits;
+            uint32_t upto = items;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t x = __shfl_up(upto, d);
+                if (lane >= d) upto += x;
+            }
+            const uint64_t at = __ballot(before + upto > item);
+            if (at) {
+                const int from = __ffsll((unsigned long long)at) - 1;
+                const uint32_t i = item - before - (__shfl(upto, from) - __shfl(items, from));
+                const uint32_t its = __shfl(splits, from);
+                seq = __builtin_amdgcn_readfirstlane(s0 + from);
+                // the last tiles of a sequence see the most keys: they go first
+                tile = __builtin_amdgcn_readfirstlane(__shfl(tiles, from) - 1 - i / its);
+                split = __builtin_amdgcn_readfirstlane(i % its);
+            }
+            before += __shfl(upto, 63);
+        }
+    }
 };
 
 typedef __attribute__((address_space(3))) void* lds_void;
@@ -460,22 +551,21 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
     __shared__ __align__(1024) short lds_k[2][kKeys * D];
     __shared__ __align__(1024) short lds_v[2][kKeys * D];
 
-    const int head = blockIdx.x % a.kv_heads;
-    const int group = a.q_heads / a.kv_heads;
-    // the last tiles of a sequence see the most keys: they go first
-    const int tile = gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads;
-    const Sequence seq = read_sequence(a, blockIdx.y);
-    const int rows = seq.tokens * group;
-    const int row0 = tile * C::kRows;
-    if (rows <= kRows || row0 >= rows) return;
+    TileWork<D> work(a, plan);
+    if (plan.splits > 1 && blockIdx.x == 0 && threadIdx.x == 0) *(uint32_t*)((char*)a.workspace + plan.offset) = work.chunk;
+    work.find(a, blockIdx.x / a.kv_heads);
+    if (work.seq < 0) return;
+    const int head = blockIdx.x % a.kv_heads, group = a.q_heads / a.kv_heads;
+    const Sequence seq = read_sequence<Table>(a, work.seq);
+    const int rows = seq.tokens * group, row0 = work.tile * C::kRows;
     const int row_end = min(row0 + C::kRows, rows);
     const int base = seq.keys - seq.tokens;   // position of token 0
     const int p_low = base + row0 / group, p_high = base + (row_end - 1) / group;
     const int window = (int)a.window, sinks = (int)a.sinks;
     const Steps steps(kKeys, p_low, p_high, window, sinks);
-    const int begin = blockIdx.z * plan.chunk, end = min(begin + (int)plan.chunk, steps.count);
-    if (blockIdx.z && begin >= end) return;
-    const bool whole = steps.count <= (int)plan.chunk;   // no other split of this tile
+    const int begin = work.split * (int)work.chunk, end = min(begin + (int)work.chunk, steps.count);
+    if (work.split && begin >= end) return;
+    const bool whole = steps.count <= (int)work.chunk;   // no other split of this tile
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
@@ -493,7 +583,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) q[i] = *(const s16x8*)(p + 16 * i);
     }
-    const Table table = (Table)(a.page_table + blockIdx.y * a.table_stride);
+    const Table table = (Table)(a.page_table + work.seq * a.table_stride);
     const float scale = a.scale * kLog2e;
 
     // Loads of a tile: load i of a wave brings the rows kLoadRows (wave + kWaves i) + lane / kChunks. With pages of 16
@@ -697,7 +787,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
     l += __shfl_xor(l, 32);
     const int64_t at = (int64_t)(seq.first + token) * a.q_heads + q_head;
     const int64_t part_rows = (int64_t)a.tokens * a.q_heads;
-    float* parts = (float*)((char*)a.workspace + plan.offset) + blockIdx.z * part_rows * (D + 2);
+    float* parts = (float*)((char*)a.workspace + plan.offset + kPartsAt) + work.split * part_rows * (D + 2);
     if (wave_row + col < row_end) {
         if (whole) {
             const float inv = l > 0.0f ? 1.0f / l : l;   // NaN stays NaN
@@ -743,15 +833,12 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
     }
 }
 
-// Joins the parts of split tiles, a wave a row, in the order of the splits.
+// Joins the parts of split tiles in the order of the splits: a workgroup a token, a wave a row.
 template <class T, int D>
-__global__ __launch_bounds__(256) void attention_join_kernel(const ls_hip_attention a, const TilePlan plan) {
+__global__ __launch_bounds__(1024) void attention_join_kernel(const ls_hip_attention a, const TilePlan plan) {
     constexpr int kLane = D / 64;
     typedef float lane_sums __attribute__((ext_vector_type(kLane)));
-    const int64_t at = blockIdx.x * 4ll + (threadIdx.x >> 6), part_rows = (int64_t)a.tokens * a.q_heads;
-    if (at >= part_rows) return;
-    const int lane = threadIdx.x & 63, t = (int)(at / a.q_heads), q_head = (int)(at % a.q_heads);
-    const int group = a.q_heads / a.kv_heads;
+    const int lane = threadIdx.x & 63, t = blockIdx.x, group = a.q_heads / a.kv_heads;
     // the sequence of token t: the last one that starts at or before it
     int s = 0;
     for (int s0 = 0; s0 < (int)a.sequences; s0 += 64) {
@@ -759,29 +846,35 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const ls_hip_attent
         if (!before) break;
         s = s0 + 63 - __clzll((long long)before);
     }
-    const Sequence seq = read_sequence(a, __builtin_amdgcn_readfirstlane(s));
-    const int rows = seq.tokens * group;
+    const Sequence seq = read_sequence<Table>(a, __builtin_amdgcn_readfirstlane(s));
+    const int rows = seq.tokens * group, base = seq.keys - seq.tokens;
     if (rows <= kRows || t < seq.first || t >= seq.first + seq.tokens) return;
-    const int row0 = ((t - seq.first) * group + q_head % group) / Tile<D>::kRows * Tile<D>::kRows;
-    const int row_end = min(row0 + Tile<D>::kRows, rows), base = seq.keys - seq.tokens;
-    const Steps steps(Tile<D>::kKeys, base + row0 / group, base + (row_end - 1) / group, (int)a.window, (int)a.sinks);
-    if (steps.count <= (int)plan.chunk) return;   // one split: the result is written
-    const float* parts = (const float*)((const char*)a.workspace + plan.offset);
-    lane_sums o = {};
-    float m = kNoKey, l = 0.0f;
-    for (int begin = 0; begin < steps.count; begin += plan.chunk, parts += part_rows * (D + 2)) {
-        const f32x2 ml = *(const f32x2*)(parts + part_rows * D + 2 * at);
-        const lane_sums x = *(const lane_sums*)(parts + at * D + kLane * lane);
-        const float next = fmaxf(m, ml[0]), old = __builtin_amdgcn_exp2f(m - next), f = __builtin_amdgcn_exp2f(ml[0] - next);
-        o = o * old + x * f;
-        l = l * old + ml[1] * f;
-        m = next;
-    }
-    const float inv = l > 0.0f ? 1.0f / l : l;   // NaN stays NaN
-    short* out = (short*)a.out + (int64_t)t * a.out_token_stride + q_head * a.out_head_stride + kLane * lane;
+    const int chunk = *(const int*)((const char*)a.workspace + plan.offset);
+    const int64_t part_rows = (int64_t)a.tokens * a.q_heads;
+    for (int q_head = threadIdx.x >> 6; q_head < (int)a.q_heads; q_head += 16) {
+        const int row0 = ((t - seq.first) * group + q_head % group) / Tile<D>::kRows * Tile<D>::kRows;
+        const int row_end = min(row0 + Tile<D>::kRows, rows);
+        const Steps steps(Tile<D>::kKeys, base + row0 / group, base + (row_end - 1) / group, (int)a.window, (int)a.sinks);
+        if (steps.count <= chunk) continue;   // one split: the result is written
+        const int64_t at = (int64_t)t * a.q_heads + q_head;
+        const float* parts = (const float*)((const char*)a.workspace + plan.offset + kPartsAt);
+        lane_sums o = {};
+        float m = kNoKey, l = 0.0f;
+#pragma unroll 4
+        for (int begin = 0; begin < steps.count; begin += chunk, parts += part_rows * (D + 2)) {
+            const f32x2 ml = *(const f32x2*)(parts + part_rows * D + 2 * at);
+            const lane_sums x = *(const lane_sums*)(parts + at * D + kLane * lane);
+            const float next = fmaxf(m, ml[0]), old = __builtin_amdgcn_exp2f(m - next), f = __builtin_amdgcn_exp2f(ml[0] - next);
+            o = o * old + x * f;
+            l = l * old + ml[1] * f;
+            m = next;
+        }
+        const float inv = l > 0.0f ? 1.0f / l : l;   // NaN stays NaN
+        short* out = (short*)a.out + (int64_t)t * a.out_token_stride + q_head * a.out_head_stride + kLane * lane;
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) out[i] = (short)T::pack(o[i] * inv, 0.0f);
-    if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+        for (int i = 0; i < kLane; ++i) out[i] = (short)T::pack(o[i] * inv, 0.0f);
+        if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
+    }
 }
 
 bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
@@ -806,15 +899,8 @@ int check(const ls_hip_attention& a) {
     if ((uint64_t)a.k_slot_stride * a.page_size > 0x3fffffffu || (uint64_t)a.v_slot_stride * a.page_size > 0x3fffffffu)
         return ENOTSUP;
     if (a.dtype == LS_TYPE_F32 || (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256)) return ENOTSUP;
-    if ((uint64_t)a.max_new * (a.q_heads / a.kv_heads) > 0x3fffffffu || a.sequences > 65535) return ENOTSUP;
+    if ((uint64_t)a.tokens * a.q_heads > 0x3fffffffu || a.sequences > 65535) return ENOTSUP;
     return 0;
-}
-
-// Steps of `unit` keys that rows of up to `span` neighbouring tokens see.
-uint64_t most_steps(const ls_hip_attention& a, uint64_t unit, uint64_t span) {
-    const uint64_t steps = (a.max_context + unit - 1) / unit;
-    if (!a.window) return steps;
-    return std::min(steps, (a.window + span + unit - 1) / unit + 1 + (a.sinks + unit - 1) / unit);
 }
 
 // Splits of the sequences that take the row kernel: enough workgroups to fill the card, none with less than a
@@ -822,7 +908,7 @@ uint64_t most_steps(const ls_hip_attention& a, uint64_t unit, uint64_t span) {
 SplitPlan plan_rows(const ls_hip_attention& a) {
     SplitPlan p{};
     p.rows = (uint32_t)std::min<uint64_t>((uint64_t)a.max_new * (a.q_heads / a.kv_heads), kRows);
-    const uint64_t steps = most_steps(a, kStepKeys, kRows), groups = (uint64_t)a.sequences * a.kv_heads;
+    const uint64_t steps = most_steps(a.max_context, kStepKeys, kRows, a.window, a.sinks), groups = (uint64_t)a.sequences * a.kv_heads;
     const uint64_t chunk = std::max<uint64_t>(1, (steps * groups + kFill - 1) / kFill);
     p.chunk = (uint32_t)std::min<uint64_t>((chunk + kRowWaves - 1) / kRowWaves * kRowWaves, 1u << 30);
     p.splits = (uint32_t)std::max<uint64_t>(1, (steps + p.chunk - 1) / p.chunk);
@@ -830,19 +916,22 @@ SplitPlan plan_rows(const ls_hip_attention& a) {
     return p;
 }
 
-// Splits of the tiles: two workgroups a compute unit if the tokens at hand all belong to chunks, none with less than 8
-// steps (its part of the sums costs as much as one).
-TilePlan plan_tiles(const ls_hip_attention& a, uint32_t tile_rows, uint32_t tile_keys, uint64_t offset) {
+// Room for the splits of the tiles, as if all tokens belonged to few chunks.
+TilePlan plan_tiles(const ls_hip_attention& a, uint64_t tile_rows, uint64_t tile_keys, uint64_t offset) {
     TilePlan p{};
-    const uint64_t group = a.q_heads / a.kv_heads, rows = a.tokens * group;
-    const uint64_t tiles = rows / tile_rows + std::min<uint64_t>(a.sequences, rows / (kRows + 1) + 1);
-    const uint64_t steps = most_steps(a, tile_keys, tile_rows / group + 2);
-    const uint64_t splits = std::max<uint64_t>(1, 512 / (tiles * a.kv_heads));
-    p.chunk = (uint32_t)std::max<uint64_t>(8, (steps + splits - 1) / splits);
-    p.splits = (uint32_t)std::max<uint64_t>(1, (steps + p.chunk - 1) / p.chunk);
+    const uint64_t group = a.q_heads / a.kv_heads;
+    const uint64_t least = std::max<uint64_t>(1, a.tokens * group / tile_rows) * a.kv_heads;   // workgroups without splits
+    const uint64_t steps = most_steps(a.max_context, tile_keys, tile_rows / group + 2, a.window, a.sinks);
+    p.splits = (uint32_t)std::max<uint64_t>(1, std::min(kTileFill / least, (steps + kLeastChunk - 1) / kLeastChunk));
     p.offset = (offset + 255) / 256 * 256;
-    if (p.splits > 1) p.bytes = p.offset + p.splits * (uint64_t)a.tokens * a.q_heads * (a.head_dim + 2) * sizeof(float);
+    if (p.splits > 1) p.bytes = p.offset + kPartsAt + p.splits * (uint64_t)a.tokens * a.q_heads * (a.head_dim + 2) * sizeof(float);
     return p;
+}
+// Workgroups of the tiles: every tile ends with a split that is not full.
+uint32_t tile_grid(const ls_hip_attention& a, uint64_t tile_rows) {
+    const uint64_t rows = (uint64_t)a.tokens * (a.q_heads / a.kv_heads);
+    const uint64_t tiles = rows / tile_rows + std::min<uint64_t>(a.sequences, rows / (kRows + 1));
+    return (uint32_t)((tiles + kTileFill / a.kv_heads + 1) * a.kv_heads);
 }
 
 struct Plan {
@@ -874,12 +963,11 @@ void launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
     }
     if (plan.by_tiles) {
         typedef Tile<D> C;
-        const uint32_t rows = a.max_new * (a.q_heads / a.kv_heads);
-        const dim3 grid((rows + C::kRows - 1) / C::kRows * a.kv_heads, a.sequences, plan.tiles.splits);
+        const uint32_t grid = tile_grid(a, C::kRows);
         if (a.page_size >= 16) attention_tile_kernel<T, D, true><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
         else attention_tile_kernel<T, D, false><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
         if (plan.tiles.splits > 1)
-            attention_join_kernel<T, D><<<(uint32_t)(((uint64_t)a.tokens * a.q_heads + 3) / 4), 256, 0, stream>>>(a, plan.tiles);
+            attention_join_kernel<T, D><<<a.tokens, 1024, 0, stream>>>(a, plan.tiles);
     }
 }
 
