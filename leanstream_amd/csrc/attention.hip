@@ -139,6 +139,7 @@ struct Steps {
 constexpr int kRowWaves = 4;
 constexpr int kRows = 16;          // sequences of up to this many rows go this way
 constexpr int kStepKeys = 32;
+constexpr uint32_t kMaxSplits = 128;   // one workgroup joins them
 
 struct SplitPlan {
     uint32_t splits;       // of the longest sequence
@@ -153,11 +154,10 @@ constexpr uint32_t kFill = 1024;   // workgroups that fill the card, 4 on each o
 constexpr uint64_t kCounterBytes = kFill * sizeof(uint32_t);
 
 __device__ __forceinline__ void store_agent(float* p, float a, float b) {
-    typedef float v2 __attribute__((ext_vector_type(2)));
-    __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, v2{a, b}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, f32x2{a, b}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float load_agent(const float* p) {
-    return __uint_as_float(__hip_atomic_load((const uint32_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+__device__ __forceinline__ f32x2 load_agent(const float* p) {
+    return __builtin_bit_cast(f32x2, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
 // The 32 keys of a step: where they lie. Pages of 16 keys and more: both halves lie in one page each, their
@@ -349,6 +349,12 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
     const uint32_t stride = plan.rows * (D + 2);   // floats of a split: rows of sums, then m and l of every row
     float* space = (float*)((char*)a.workspace + kCounterBytes) + (uint64_t)pair * plan.splits * stride;
     const int items = rows * (D / 2);
+    auto put = [&](int r, int c, float x, float y, float top, float sum) {
+        const int64_t token = seq.first + r / group, q_head = head * group + r % group;
+        const float inv = sum > 0.0f ? 1.0f / sum : sum;   // NaN stays NaN
+        *(uint32_t*)((short*)a.out + token * a.out_token_stride + q_head * a.out_head_stride + c) = T::pack(x * inv, y * inv);
+        if (a.lse && c == 0) a.lse[token * a.q_heads + q_head] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
+    };
     for (int i = threadIdx.x; i < items; i += 64 * kRowWaves) {
         const int r = i / (D / 2), c = 2 * (i % (D / 2));
         float top = lds_m[0][r];
@@ -367,11 +373,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
             store_agent(part + r * D + c, x, y);
             if (c == 0) store_agent(part + plan.rows * D + 2 * r, top, sum);
         } else {
-            const int token = seq.first + r / group, q_head = head * group + r % group;
-            const float inv = sum > 0.0f ? 1.0f / sum : sum;   // NaN stays NaN
-            *(uint32_t*)((short*)a.out + token * a.out_token_stride + q_head * a.out_head_stride + c) = T::pack(x * inv, y * inv);
-            if (a.lse && c == 0)
-                a.lse[(int64_t)token * a.q_heads + q_head] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
+            put(r, c, x, y, top, sum);
         }
     }
     if (splits == 1) return;
@@ -389,23 +391,31 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
     }
     __syncthreads();
     if (lds_turn != (uint32_t)splits - 1) return;
-    for (int i = threadIdx.x; i < rows * D; i += 64 * kRowWaves) {
-        const int r = i / D, c = i % D;
-        float top = kNoKey, x = 0.0f, sum = 0.0f;
-        for (int s = 0; s < splits; ++s) {
-            const float* part = space + s * stride;
-            const float ms = load_agent(part + plan.rows * D + 2 * r);
-            const float next = fmaxf(top, ms);
-            const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(ms - next);
-            x = x * old + load_agent(part + r * D + c) * f;
-            sum = sum * old + load_agent(part + plan.rows * D + 2 * r + 1) * f;
-            top = next;
+    // m and l of every split and row, then the columns pairwise, eight splits' loads at a time
+    f32x2* ml = (f32x2*)&lds_o[0][0][0];
+    static_assert(kMaxSplits * kRows * sizeof(f32x2) <= sizeof(lds_o), "room");
+    for (int i = threadIdx.x; i < splits * rows; i += 64 * kRowWaves)
+        ml[i] = load_agent(space + i / rows * stride + plan.rows * D + 2 * (i % rows));
+    __syncthreads();
+    for (int i = threadIdx.x; i < items; i += 64 * kRowWaves) {
+        const int r = i / (D / 2), c = 2 * (i % (D / 2));
+        float top = kNoKey, x = 0.0f, y = 0.0f, sum = 0.0f;
+        for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[s * rows + r][0]);
+        for (int s0 = 0; s0 < splits; s0 += 8) {
+            f32x2 part[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) part[s] = load_agent(space + min(s0 + s, splits - 1) * stride + r * D + c);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                if (s0 + s >= splits) break;
+                const f32x2 its = ml[(s0 + s) * rows + r];
+                const float f = __builtin_amdgcn_exp2f(its[0] - top);
+                x += part[s][0] * f;
+                y += part[s][1] * f;
+                sum += its[1] * f;
+            }
         }
-        const int token = seq.first + r / group, q_head = head * group + r % group;
-        const float inv = sum > 0.0f ? 1.0f / sum : sum;
-        ((short*)a.out)[token * a.out_token_stride + q_head * a.out_head_stride + c] = (short)T::pack(x * inv, 0.0f);
-        if (a.lse && c == 0)
-            a.lse[(int64_t)token * a.q_heads + q_head] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
+        put(r, c, x, y, top, sum);
     }
 }
 
@@ -833,7 +843,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
     }
 }
 
-// Joins the parts of split tiles in the order of the splits: a workgroup a token, a wave a row.
+// Joins the parts of split tiles in the order of the splits: a workgroup 16 heads of a token, a wave a row.
 template <class T, int D>
 __global__ __launch_bounds__(1024) void attention_join_kernel(const ls_hip_attention a, const TilePlan plan) {
     constexpr int kLane = D / 64;
@@ -851,16 +861,17 @@ __global__ __launch_bounds__(1024) void attention_join_kernel(const ls_hip_atten
     if (rows <= kRows || t < seq.first || t >= seq.first + seq.tokens) return;
     const int chunk = *(const int*)((const char*)a.workspace + plan.offset);
     const int64_t part_rows = (int64_t)a.tokens * a.q_heads;
-    for (int q_head = threadIdx.x >> 6; q_head < (int)a.q_heads; q_head += 16) {
+    const int q_head = 16 * blockIdx.y + (threadIdx.x >> 6);
+    if (q_head < (int)a.q_heads) {
         const int row0 = ((t - seq.first) * group + q_head % group) / Tile<D>::kRows * Tile<D>::kRows;
         const int row_end = min(row0 + Tile<D>::kRows, rows);
         const Steps steps(Tile<D>::kKeys, base + row0 / group, base + (row_end - 1) / group, (int)a.window, (int)a.sinks);
-        if (steps.count <= chunk) continue;   // one split: the result is written
+        if (steps.count <= chunk) return;   // one split: the result is written
         const int64_t at = (int64_t)t * a.q_heads + q_head;
         const float* parts = (const float*)((const char*)a.workspace + plan.offset + kPartsAt);
         lane_sums o = {};
         float m = kNoKey, l = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
         for (int begin = 0; begin < steps.count; begin += chunk, parts += part_rows * (D + 2)) {
             const f32x2 ml = *(const f32x2*)(parts + part_rows * D + 2 * at);
             const lane_sums x = *(const lane_sums*)(parts + at * D + kLane * lane);
@@ -909,7 +920,7 @@ SplitPlan plan_rows(const ls_hip_attention& a) {
     SplitPlan p{};
     p.rows = (uint32_t)std::min<uint64_t>((uint64_t)a.max_new * (a.q_heads / a.kv_heads), kRows);
     const uint64_t steps = most_steps(a.max_context, kStepKeys, kRows, a.window, a.sinks), groups = (uint64_t)a.sequences * a.kv_heads;
-    const uint64_t chunk = std::max<uint64_t>(1, (steps * groups + kFill - 1) / kFill);
+    const uint64_t chunk = std::max<uint64_t>(std::max<uint64_t>(1, (steps * groups + kFill - 1) / kFill), (steps + kMaxSplits - 1) / kMaxSplits);
     p.chunk = (uint32_t)std::min<uint64_t>((chunk + kRowWaves - 1) / kRowWaves * kRowWaves, 1u << 30);
     p.splits = (uint32_t)std::max<uint64_t>(1, (steps + p.chunk - 1) / p.chunk);
     if (p.splits > 1) p.bytes = kCounterBytes + groups * p.splits * p.rows * (a.head_dim + 2) * sizeof(float);
@@ -967,7 +978,7 @@ void launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
         if (a.page_size >= 16) attention_tile_kernel<T, D, true><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
         else attention_tile_kernel<T, D, false><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
         if (plan.tiles.splits > 1)
-            attention_join_kernel<T, D><<<a.tokens, 1024, 0, stream>>>(a, plan.tiles);
+            attention_join_kernel<T, D><<<dim3(a.tokens, (a.q_heads + 15) / 16), 1024, 0, stream>>>(a, plan.tiles);
     }
 }
 
