@@ -442,10 +442,11 @@ struct Tile {
     static constexpr int kChunks = D / 8;                     // 16-byte chunks of a row
     static constexpr int kLoads = kKeys * kChunks / (64 * kWaves);   // a wave's loads of a tile, 64 chunks each
     static constexpr int kLoadRows = 64 / kChunks;            // rows of one load
-    // Chunk c of row r lies at position c ^ turn(r), so that 8 rows' chunks (K operands) and 4 rows' pairs of
-    // chunks (transposing reads) lie in different banks. turn(r + 8) = turn(r) ^ 1 for r % 16 < 8.
+    // Chunk c of row r lies at position c ^ turn(r): the chunks that 16 lanes read of as many rows (K operands) and the
+    // 64 bytes that 32 lanes read of each of 4 rows (transposing reads) lie in different banks, all 64 of them
+    // (measured: no conflicts, 256 bytes a cycle). turn(r + 8) = turn(r) ^ 2 for r % 16 < 8.
     static __device__ __forceinline__ int turn(int r) {
-        return D == 64 ? (r >> 1 & 3) << 1 | (r >> 3 & 1) : (r & 7) << 1 | (r >> 3 & 1);
+        return D == 64 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3);
     }
 };
 // The running maximum moves only where a score exceeds it by more than this (base 2): until then P is at most
@@ -680,7 +681,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
         const lds_bytes lds = (lds_bytes)lds_v + (t & 1) * (2 * D * kKeys);
         typedef __attribute__((address_space(3))) s16x4* lds_ptr;
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (v_at ^ (64 * d)) + 2 * D * 16 * t16));
-        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (v_at ^ (64 * d) ^ 16) + 2 * D * (16 * t16 + 8)));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (v_at ^ (64 * d) ^ 32) + 2 * D * (16 * t16 + 8)));
         return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     auto sees_all = [&](int key0, int low, int high) {   // rows from position low to high see every key of a tile
@@ -788,7 +789,6 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
                 for (int d = 0; d < D / 32; ++d) o[d] = T::mfma32(v[t16 & 1][d], __builtin_bit_cast(s16x8, p[t16]), o[d]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) top = fmaxf(top, next[t16 / 2][t16 % 2 * 8 + i]);
-                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int kt = 0; kt < kSub; ++kt) s[kt] = next[kt];
