@@ -69,7 +69,8 @@ struct Scale {
         bins = fminf(16.0f / temperature, 3e38f);
     }
     // bin on the scale of all logits of a row, rising with the logit
-    __device__ __forceinline__ int bin(float l) const { return (int)fminf(fmaxf(floorf(l * bins), -1e9f), 1e9f); }
+    __device__ __forceinline__ float steps(float l) const { return fminf(fmaxf(floorf(l * bins), -1e9f), 1e9f); }
+    __device__ __forceinline__ int bin(float l) const { return (int)steps(l); }
     // exp((l - top) / T) 2^up for l <= top; 0 for -inf
     __device__ __forceinline__ float e(float l, float top, int up = 0) const {
         const float t = l - top;
@@ -103,6 +104,8 @@ struct Shared {
     // of the row's chunks
     double sums[kMaxChunks];
     uint64_t list[kMaxChunks];
+    double unit[kMaxChunks];
+    int shift[kMaxChunks];
     float tops[kMaxChunks];
     uint32_t held[kMaxChunks];
     uint64_t few[64];
@@ -689,18 +692,31 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
         auto cut_in_bins = [&]() LS_INLINE -> bool {
             const int row_bin = scale.bin(top);
             const double limit = (double)fmaxf(top_p, 0.0f) * row_sum;
-            // thread b: bin b of the row, chunk by chunk
+            // a chunk's bins begin `shift` bins below the row's, in units of the chunk's best token
+            if (mine) {
+                const float its = sh.tops[threadIdx.x];
+                sh.shift[threadIdx.x] = its > -INFINITY ? row_bin - scale.bin(its) : kBins;
+                sh.unit[threadIdx.x] = 0x1p-32 * (double)scale.e(its, top);
+            }
+            __syncthreads();
+            // thread b: bin b of the row, 16 chunks' loads at a time
             uint32_t n = 0;
             double w = 0.0;
-            for (uint32_t c = 0; c < rows.chunks; ++c) {
-                const int b = (int)threadIdx.x - (row_bin - scale.bin(sh.tops[c]));
-                if (!(sh.tops[c] > -INFINITY) || b < 0) continue;
-                const uint64_t x = record[c * words + kHead + rows.room + b];
-                n += (uint32_t)(x >> kCountShift);
-                w += (double)(x & ((1ull << kCountShift) - 1)) * 0x1p-32 * (double)scale.e(sh.tops[c], top);
+            for (uint32_t c0 = 0; c0 < rows.chunks; c0 += 16) {
+                uint64_t x[16];
+#pragma unroll
+                for (uint32_t c = 0; c < 16; ++c) {
+                    const uint32_t at = min(c0 + c, rows.chunks - 1);
+                    x[c] = record[at * words + kHead + rows.room + max((int)threadIdx.x - sh.shift[at], 0)];
+                }
+#pragma unroll
+                for (uint32_t c = 0; c < 16; ++c) {
+                    if (c0 + c >= rows.chunks || (int)threadIdx.x < sh.shift[c0 + c]) continue;
+                    n += (uint32_t)(x[c] >> kCountShift);
+                    w += (double)(x[c] & ((1ull << kCountShift) - 1)) * sh.unit[c0 + c];
+                }
             }
             double all_bins;
-            __syncthreads();
             const double before = block_before(w, sh.wave_sum, &all_bins);
             if (threadIdx.x == 0) sh.token = kAll, sh.turn = 0;
             __syncthreads();
@@ -712,46 +728,70 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
             __syncthreads();
             if (sh.before_count > kCandidates) return false;
             const uint64_t need = sh.before_weight;
-            // its tokens, in any order, into the slots of the candidates (which are all read)
-            const int wanted = row_bin - (int)bin;
-            auto slot_at = [&](uint32_t slot) { return record + slot / rows.room * words + kHead + slot % rows.room; };
-            auto take = [&](float v, uint32_t i) LS_INLINE {
-                if (v > -INFINITY && scale.bin(v) == wanted) {
-                    const uint32_t slot = atomicAdd(&sh.turn, 1u);
-                    if (slot < rows.room * rows.chunks) *slot_at(slot) = (uint64_t)order_of(v) << 32 | i;
-                }
-            };
-            const uint32_t whole = a.vocab / 8;
-#pragma unroll 4
-            for (uint32_t i = threadIdx.x; i < whole; i += kThreads) {
-                const typename Vec8<T>::type x = *(const typename Vec8<T>::type*)(logits + 8 * i);
+            // The ids of its tokens, in any order, into the slots of the candidates (which are all read). A thread marks
+            // what it finds among 64 logits before it takes slots: one by one, the few hits of every wave would each
+            // wait for the counter.
+            const float wanted = (float)(row_bin - (int)bin);
+            auto slot_at = [&](uint32_t slot) LS_INLINE { return record + slot / rows.room * words + kHead + slot % rows.room; };
+            constexpr uint32_t kDeep = 8;
+            const uint32_t room = rows.room * rows.chunks, whole = a.vocab / 8;
+            for (uint32_t i0 = threadIdx.x; i0 <= whole; i0 += kDeep * kThreads) {
+                typename Vec8<T>::type x[kDeep];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) take(to_float(x[j]), 8 * i + j);
+                for (uint32_t d = 0; d < kDeep; ++d) {
+                    const uint32_t i = i0 + d * kThreads;
+                    if (i < whole) x[d] = *(const typename Vec8<T>::type*)(logits + 8 * i);
+                    else
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[d][j] = 8 * i + j < a.vocab ? logits[8 * i + j] : (T)-INFINITY;
+                }
+                uint64_t hits = 0;
+#pragma unroll
+                for (uint32_t d = 0; d < kDeep; ++d)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float v = to_float(x[d][j]);
+                        hits |= (uint64_t)(scale.steps(v) == wanted && v > -INFINITY) << (8 * d + j);
+                    }
+                while (hits) {
+                    const uint32_t at = __ffsll((unsigned long long)hits) - 1, slot = atomicAdd(&sh.turn, 1u);
+                    hits &= hits - 1;
+                    if (slot < room) *slot_at(slot) = 8 * (i0 + at / 8 * kThreads) + at % 8;
+                }
             }
-            if (8 * whole + threadIdx.x < a.vocab) take(to_float(logits[8 * whole + threadIdx.x]), 8 * whole + threadIdx.x);
             __syncthreads();   // and their stores, for this workgroup
             const uint32_t held = sh.turn;
-            if (held > rows.room * rows.chunks) return false;
+            if (held > room) return false;
+            uint32_t lowest = kAll, highest = 0;
 #pragma unroll
             for (uint32_t i = 0; i < kSlots; ++i) {
-                const uint32_t slot = threadIdx.x * kSlots + i;
-                const uint64_t x = slot < held ? *slot_at(slot) : 0;
-                order[i] = (uint32_t)(x >> 32);
-                id[i] = (uint32_t)x;
-                weight[i] = x ? scale.weight(logit_of(order[i]), top) : 0;
+                const uint32_t slot = i * kThreads + threadIdx.x;
+                id[i] = slot < held ? (uint32_t)*slot_at(slot) : 0;
             }
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i) {
+                const bool in = i * kThreads + threadIdx.x < held;
+                const float v = in ? to_float(logits[id[i]]) : 0.0f;
+                order[i] = in ? order_of(v) : 0;
+                weight[i] = in ? scale.weight(v, top) : 0;
+                if (weight[i]) lowest = min(lowest, order[i]), highest = max(highest, order[i]);
+            }
+#pragma unroll
+            for (int d = 32; d; d >>= 1) {
+                lowest = min(lowest, (uint32_t)__shfl_xor(lowest, d));
+                highest = max(highest, (uint32_t)__shfl_xor(highest, d));
+            }
+            if (lane == 0) sh.wave32[wave] = lowest, sh.wave64[wave] = highest;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                lowest = min(lowest, sh.wave32[i]);
+                highest = max(highest, (uint32_t)sh.wave64[i]);
+            }
+            if (!highest) return false;
             uint64_t of_list;
-            cut = select(candidates, low, high, all, kAll, need ? need : 1, sh, &of_list);
-            if (!cut.order) {   // not reached, by a rounding of the bins' sums: all of the bin
-                if (threadIdx.x == 0) sh.token = kAll;
-                __syncthreads();
-                candidates([&](uint32_t o, uint32_t w) LS_INLINE {
-                    if (w) atomicMin(&sh.token, o);
-                });
-                __syncthreads();
-                cut = Cut{sh.token, kAll};
-                if (sh.token == kAll) return false;
-            }
+            cut = select(candidates, lowest, highest, all, kAll, need ? need : 1, sh, &of_list);
+            if (!cut.order) cut = Cut{lowest, kAll};   // not reached, by a rounding of the bins' sums: all of the bin
             if (min_p > 0.0f && !(scale.e(logit_of(cut.order), top) >= min_p)) return false;
             // kept weight of every chunk: its bins above, and what the list holds of it
             __syncthreads();
@@ -763,14 +803,15 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
                 if (weight[i] && order[i] == cut.order) atomicAdd(&sh.held[id[i] / kChunk], 1u);
             }
             for (uint32_t c = wave; c < rows.chunks; c += kWaves) {
-                const float ctop = sh.tops[c];
+                const uint64_t* bins = record + c * words + kHead + rows.room;
+                const int above = (int)bin - sh.shift[c];
                 double x = 0.0;
-                if (ctop > -INFINITY) {
-                    const uint64_t* bins = record + c * words + kHead + rows.room;
-                    const int shift = row_bin - scale.bin(ctop);
-                    for (int b = (int)lane; b < (int)bin - shift; b += 64) x += (double)(bins[b] & ((1ull << kCountShift) - 1));
-                    x *= 0x1p-32 * (double)scale.e(ctop, top);
+#pragma unroll
+                for (int b = 0; b < kBins; b += 64) {
+                    const uint64_t w = bins[b + lane];
+                    if (b + (int)lane < above) x += (double)(w & ((1ull << kCountShift) - 1));
                 }
+                x *= sh.unit[c];
 #pragma unroll
                 for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
                 if (lane == 0) sh.sums[c] = x;
