@@ -36,6 +36,7 @@ constexpr uint32_t kChunkCandidates = 256; // of a chunk, at most
 constexpr uint32_t kRowBlock = 256;        // rows of a launch
 constexpr int kBins = 512;                 // steps of T / 16 down from a chunk's best logit: weights to e^-32
 constexpr int kCountShift = 46;            // a bin: count << 46 | weight (at most 2^13 tokens of up to 2^32)
+constexpr uint64_t kWeight = (1ull << kCountShift) - 1;
 constexpr uint32_t kAll = 0xffffffffu;
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -71,6 +72,15 @@ struct Scale {
     // bin on the scale of all logits of a row, rising with the logit
     __device__ __forceinline__ float steps(float l) const { return fminf(fmaxf(floorf(l * bins), -1e9f), 1e9f); }
     __device__ __forceinline__ int bin(float l) const { return (int)steps(l); }
+    // the smallest logit of bin b or above: a few units in the last place around b / bins
+    __device__ __forceinline__ float first_of(int b) const {
+        if (b <= -1000000000) return -INFINITY;
+        if (b > 1000000000) return INFINITY;
+        float v = (float)b / bins;
+        for (int i = 0; i < 4 && steps(v) >= (float)b; ++i) v = nextafterf(v, -INFINITY);
+        for (int i = 0; i < 8 && !(steps(v) >= (float)b); ++i) v = nextafterf(v, INFINITY);
+        return v;
+    }
     // exp((l - top) / T) 2^up for l <= top; 0 for -inf
     __device__ __forceinline__ float e(float l, float top, int up = 0) const {
         const float t = l - top;
@@ -150,9 +160,9 @@ __device__ __forceinline__ V block_before(V x, V* scratch, V* total) {
 
 // The shortest prefix within `limit` whose count reaches need_count or whose weight reaches need_weight, of the
 // tokens with an order in [base, high] that each(f) hands to f(order, weight); all of `limit` if none does.
-// kept: the weight of that prefix. A limit with fewer ties than there are must weigh need_weight. Every pass counts the 256 equal parts of the range and goes on with the one
+// kept: the weight of that prefix. Few: of at most 2^13 tokens, whose count and weight go into one word. A limit with fewer ties than there are must weigh need_weight. Every pass counts the 256 equal parts of the range and goes on with the one
 // in which a sum is reached, until it is one logit or holds so few tokens that one wave ranks them.
-template <class Each>
+template <bool Few, class Each>
 __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t high, Cut limit, uint32_t need_count,
                                       uint64_t need_weight, Shared& sh, uint64_t* kept) {
     uint64_t before_weight = 0;
@@ -165,8 +175,9 @@ __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t 
         __syncthreads();
         each([&](uint32_t order, uint32_t weight) LS_INLINE {
             if (!weight || order < base || order > high) return;
-            atomicAdd(&sh.counts[(order - base) >> shift], 1u);
-            atomicAdd((unsigned long long*)&sh.weights[(order - base) >> shift], (unsigned long long)weight);
+            const uint32_t part = (order - base) >> shift;
+            if constexpr (!Few) atomicAdd(&sh.counts[part], 1u);
+            atomicAdd((unsigned long long*)&sh.weights[part], (Few ? 1ull << kCountShift : 0) + weight);
         });
         __syncthreads();
         // The first part from above at which one of the sums is reached: a lane takes four. Where a part is one
@@ -178,8 +189,9 @@ __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t d = 255 - 4 * lane - i;
-                n[i] = sh.counts[d];
                 w[i] = sh.weights[d];
+                n[i] = Few ? (uint32_t)(w[i] >> kCountShift) : sh.counts[d];
+                if (Few) w[i] &= kWeight;
                 if (shift == 0 && base + d == limit.order && n[i] > limit.ties) w[i] = w[i] / n[i] * limit.ties, n[i] = limit.ties;
                 c += n[i];
                 s += w[i];
@@ -210,9 +222,9 @@ __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t 
             *kept = before_weight;
             return limit;
         }
-        uint32_t n = sh.counts[digit];
+        uint32_t n = Few ? (uint32_t)(sh.weights[digit] >> kCountShift) : sh.counts[digit];
         if (shift == 0) {
-            const uint64_t one = sh.weights[digit] / n;
+            const uint64_t one = (Few ? sh.weights[digit] & kWeight : sh.weights[digit]) / n;
             if (base + digit == limit.order) n = min(n, limit.ties);
             // ties needed for the count and for the weight, whichever is reached first
             const uint64_t ties = min(min((uint64_t)n, (uint64_t)need_count), (need_weight - 1) / one + 1);
@@ -501,14 +513,18 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
         for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
         if (lane == 0) sh.wave_sum[wave] = sum;
     } else if (!greedy && filtered) {
+        // few of a wave's logits exceed the mean: they are marked first and then taken together
+        uint32_t hits = 0;
 #pragma unroll
         for (int v = 0; v < Vecs; ++v)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = l[v][j];
-                const int down = top_bin - scale.bin(x);
-                if (x > mean && down < kBins) atomicAdd((unsigned long long*)&sh.bins[down], 1ull << kCountShift);
-            }
+            for (int j = 0; j < 8; ++j) hits |= (uint32_t)(l[v][j] > mean) << (8 * v + j);
+        while (hits) {
+            const uint32_t at = __ffs(hits) - 1;
+            hits &= hits - 1;
+            const int down = top_bin - scale.bin(to_float(logits[begin + 8 * (at / 8 * kThreads + threadIdx.x) + at % 8]));
+            if (down < kBins) atomicAdd((unsigned long long*)&sh.bins[down], 1ull << kCountShift);
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -538,15 +554,16 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
         if (binned)
             for (int i = threadIdx.x; i < kBins; i += kThreads) record[kHead + rows.room + i] = sh.bins[i];
         float outside = -INFINITY;
+        const float least = scale.first_of(top_bin - bins + 1);
 #pragma unroll
         for (int v = 0; v < Vecs; ++v) {
             uint32_t mark = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float x = l[v][j];
-                if (!(x > -INFINITY)) continue;
-                if (top_bin - scale.bin(x) < bins) mark |= 1u << j;
-                else outside = fmaxf(outside, x);
+                const bool in = x >= least && x > -INFINITY;
+                mark |= (uint32_t)in << j;
+                outside = fmaxf(outside, in ? -INFINITY : x);
             }
             marks[v * kThreads + threadIdx.x] = (uint8_t)mark;
         }
@@ -647,14 +664,18 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
         // ---- candidates, in order of id: slots thread * kSlots + i
         constexpr uint32_t kSlots = kCandidates / kThreads;
         uint32_t order[kSlots], id[kSlots], weight[kSlots];
+        uint64_t slots[kSlots];
+        uint32_t chunk = threadIdx.x * kSlots / rows.room, at = threadIdx.x * kSlots % rows.room;
 #pragma unroll
         for (uint32_t i = 0; i < kSlots; ++i) {
-            const uint32_t slot = threadIdx.x * kSlots + i, chunk = slot / rows.room, at = slot % rows.room;
-            uint64_t x = 0;
-            if (chunk < rows.chunks && at < sh.held[chunk]) x = record[chunk * words + kHead + at];
-            order[i] = (uint32_t)(x >> 32);
-            id[i] = (uint32_t)x;
-            weight[i] = x ? scale.weight(logit_of(order[i]), top) : 0;
+            slots[i] = chunk < rows.chunks && at < sh.held[chunk] ? record[chunk * words + kHead + at] : 0;
+            if (++at == rows.room) at = 0, ++chunk;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) {
+            order[i] = (uint32_t)(slots[i] >> 32);
+            id[i] = (uint32_t)slots[i];
+            weight[i] = slots[i] ? scale.weight(logit_of(order[i]), top) : 0;
         }
         // what is no candidate does not matter if it weighs nothing
         // orders below this weigh nothing
@@ -675,13 +696,13 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
         uint64_t total = (uint64_t)(row_sum * 4294967296.0);
         bool known = by_count || by_weight || !edge;   // every kept token is a candidate
         if (by_count) {
-            cut = select(candidates, max(low, edge + 1), high, cut, set.top_k, ~0ull, sh, &total);
+            cut = select<true>(candidates, max(low, edge + 1), high, cut, set.top_k, ~0ull, sh, &total);
             known = above(cut);
         }
         const bool open = !known && by_weight;   // the weight that top-p takes its share of is not known
         if (by_weight && known) {
             const uint64_t limit = share(total, top_p, true);
-            cut = select(candidates, max(low, edge + 1), high, cut, kAll, limit ? limit : 1, sh, &total);
+            cut = select<true>(candidates, max(low, edge + 1), high, cut, kAll, limit ? limit : 1, sh, &total);
             known = above(cut);
         }
         // Where the cut lies below, min-p may still leave out whatever is no candidate: it then decides alone.
@@ -713,7 +734,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
                 for (uint32_t c = 0; c < 16; ++c) {
                     if (c0 + c >= rows.chunks || (int)threadIdx.x < sh.shift[c0 + c]) continue;
                     n += (uint32_t)(x[c] >> kCountShift);
-                    w += (double)(x[c] & ((1ull << kCountShift) - 1)) * sh.unit[c0 + c];
+                    w += (double)(x[c] & kWeight) * sh.unit[c0 + c];
                 }
             }
             double all_bins;
@@ -731,7 +752,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
             // The ids of its tokens, in any order, into the slots of the candidates (which are all read). A thread marks
             // what it finds among 64 logits before it takes slots: one by one, the few hits of every wave would each
             // wait for the counter.
-            const float wanted = (float)(row_bin - (int)bin);
+            const float least = scale.first_of(row_bin - (int)bin), beyond = scale.first_of(row_bin - (int)bin + 1);
             auto slot_at = [&](uint32_t slot) LS_INLINE { return record + slot / rows.room * words + kHead + slot % rows.room; };
             constexpr uint32_t kDeep = 8;
             const uint32_t room = rows.room * rows.chunks, whole = a.vocab / 8;
@@ -751,7 +772,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float v = to_float(x[d][j]);
-                        hits |= (uint64_t)(scale.steps(v) == wanted && v > -INFINITY) << (8 * d + j);
+                        hits |= (uint64_t)(v >= least && v < beyond) << (8 * d + j);
                     }
                 while (hits) {
                     const uint32_t at = __ffsll((unsigned long long)hits) - 1, slot = atomicAdd(&sh.turn, 1u);
@@ -790,7 +811,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
             }
             if (!highest) return false;
             uint64_t of_list;
-            cut = select(candidates, lowest, highest, all, kAll, need ? need : 1, sh, &of_list);
+            cut = select<true>(candidates, lowest, highest, all, kAll, need ? need : 1, sh, &of_list);
             if (!cut.order) cut = Cut{lowest, kAll};   // not reached, by a rounding of the bins' sums: all of the bin
             if (min_p > 0.0f && !(scale.e(logit_of(cut.order), top) >= min_p)) return false;
             // kept weight of every chunk: its bins above, and what the list holds of it
@@ -809,7 +830,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
 #pragma unroll
                 for (int b = 0; b < kBins; b += 64) {
                     const uint64_t w = bins[b + lane];
-                    if (b + (int)lane < above) x += (double)(w & ((1ull << kCountShift) - 1));
+                    if (b + (int)lane < above) x += (double)(w & kWeight);
                 }
                 x *= sh.unit[c];
 #pragma unroll
@@ -864,10 +885,10 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
             kept = bin_kept;
         } else {
             cut = all;
-            if (by_count || by_weight) cut = select(everything, low, high, cut, by_count ? set.top_k : kAll, ~0ull, sh, &total);
+            if (by_count || by_weight) cut = select<false>(everything, low, high, cut, by_count ? set.top_k : kAll, ~0ull, sh, &total);
             if (by_weight) {
                 const uint64_t limit = share(total, top_p, true);
-                cut = select(everything, low, high, cut, kAll, limit ? limit : 1, sh, &total);
+                cut = select<false>(everything, low, high, cut, kAll, limit ? limit : 1, sh, &total);
             }
             draw_from_row(logits, a.vocab, top, scale, cut, min_p, a.uniform[r], sh, &token, &sum64);
             kept = (double)sum64 * 0x1p-32;
