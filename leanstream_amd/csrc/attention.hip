@@ -11,6 +11,7 @@
 #include <cerrno>
 #include <cmath>
 #include "leanstream_hip.h"
+#include "wave_ops.h"
 
 // Closures over register arrays are inlined, or the arrays would lie in memory.
 #define LS_INLINE __attribute__((always_inline))
@@ -100,6 +101,24 @@ __device__ __forceinline__ Sequence read_sequence(const ls_hip_attention& a, int
 
 __device__ __forceinline__ bool sees(int key, int pos, int window, int sinks) {
     return key <= pos && (window == 0 || key > pos - window || key < sinks);
+}
+
+// Of the lanes i and i ^ 32 (i ^ 16): the larger value, the sum.
+__device__ __forceinline__ float max32(float x) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ __forceinline__ float max16(float x) {
+    const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ __forceinline__ float sum32(float x) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
+__device__ __forceinline__ float sum16(float x) {
+    const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
 }
 
 // Whether one of eight values is an infinity or NaN.
@@ -290,8 +309,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j / 4][j % 4] *= scale);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
+            top = max32(max16(top));
             const float keep = __builtin_amdgcn_exp2f(m - top);
             m = top;
             // P is rounded to the values' type for the matrix product; the sum takes it in fp32
@@ -332,8 +350,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
             if (!more) break;
         }
     }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    l = sum32(sum16(l));
 
     // the waves' sums, in their order
     if (g == 0) lds_m[wave][i16] = m, lds_l[wave][i16] = l;
@@ -469,12 +486,6 @@ __host__ __device__ inline uint64_t most_steps(uint64_t keys, uint64_t unit, uin
     return window && some < steps ? some : steps;
 }
 
-__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-    return __builtin_amdgcn_readfirstlane(x);
-}
-
 // The tiles of all sequences and their splits. Only the device knows the lengths, so every wave reads them, 64 sequences
 // at a time. `chunk`, the steps of a split, is the least that makes no more than kTileFill workgroups: a second round
 // for a few of them costs more than it shortens the first, and so do parts of sums for tiles that fill the card by
@@ -504,9 +515,7 @@ struct TileWork {
             longest = max(longest, steps);
         }
         tiles = wave_sum(tiles) * a.kv_heads;
-#pragma unroll
-        for (int d = 32; d; d >>= 1) longest = max(longest, (uint32_t)__shfl_xor(longest, d));
-        longest = __builtin_amdgcn_readfirstlane(longest);
+        longest = wave_max(longest, 0u);
         chunk = max(longest, 1u);
         if (plan.splits == 1 || 2 * tiles > kTileFill) return;
         // fewer than 2^8 tiles of fewer than 2^24 steps
@@ -529,23 +538,17 @@ struct TileWork {
             uint32_t steps;
             const uint32_t tiles = tiles_of(a, s0 + lane, &steps);
             const uint32_t splits = max(1u, (steps + chunk - 1) / chunk), items = tiles * splits;
-            uint32_t upto = items;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t x = __shfl_up(upto, d);
-                if (lane >= d) upto += x;
-            }
+            const uint32_t upto = wave_upto(items);
             const uint64_t at = __ballot(before + upto > item);
             if (at) {
                 const int from = __ffsll((unsigned long long)at) - 1;
-                const uint32_t i = item - before - (__shfl(upto, from) - __shfl(items, from));
-                const uint32_t its = __shfl(splits, from);
-                seq = __builtin_amdgcn_readfirstlane(s0 + from);
+                const uint32_t i = item - before - from_lane(upto - items, from), its = from_lane(splits, from);
+                seq = s0 + from;
                 // the last tiles of a sequence see the most keys: they go first
-                tile = __builtin_amdgcn_readfirstlane(__shfl(tiles, from) - 1 - i / its);
-                split = __builtin_amdgcn_readfirstlane(i % its);
+                tile = from_lane(tiles, from) - 1 - i / its;
+                split = i % its;
             }
-            before += __shfl(upto, 63);
+            before += from_lane(upto, 63);
         }
     }
 };
@@ -753,7 +756,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
                         if (!sees(key0 + 32 * kt + 8 * (i / 4) + 4 * h + i % 4, pos, window, sinks)) s[kt][i] = -INFINITY;
                 top = largest(s);
             }
-            top = fmaxf(top, __shfl_xor(top, 32)) * scale;
+            top = max32(top) * scale;
             if (__any(top > m + kSlack)) {
                 const float next_m = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - next_m);
                 m = next_m;
@@ -794,7 +797,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(co
             for (int kt = 0; kt < kSub; ++kt) s[kt] = next[kt];
         }
     }
-    l += __shfl_xor(l, 32);
+    l = sum32(l);
     const int64_t at = (int64_t)(seq.first + token) * a.q_heads + q_head;
     const int64_t part_rows = (int64_t)a.tokens * a.q_heads;
     float* parts = (float*)((char*)a.workspace + plan.offset + kPartsAt) + work.split * part_rows * (D + 2);

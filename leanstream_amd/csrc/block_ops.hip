@@ -6,6 +6,7 @@
 #include <cerrno>
 #include <cmath>
 #include "leanstream_hip.h"
+#include "wave_ops.h"
 
 namespace lsamd {
 namespace {
@@ -50,8 +51,7 @@ __device__ __forceinline__ void store8(T* row, uint32_t i, uint32_t width, const
 // Sum over the waves of a row.
 template <int Waves>
 __device__ __forceinline__ float row_sum(float x, float* scratch) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+    x = wave_sum(x);
     if constexpr (Waves > 1) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;

@@ -20,6 +20,7 @@
 #include <algorithm>
 #include <cerrno>
 #include "leanstream_hip.h"
+#include "wave_ops.h"
 
 // Arrays that a closure reaches stay in registers only where it is inlined.
 #define LS_INLINE __attribute__((always_inline))
@@ -127,21 +128,6 @@ struct ChunkShared {
     uint32_t wave32[kWaves], digit;
 };
 
-__device__ __forceinline__ uint64_t wave_max(uint64_t x) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) x = max(x, (uint64_t)__shfl_xor((unsigned long long)x, d));
-    return x;
-}
-template <class V>
-__device__ __forceinline__ V wave_upto(V x) {   // inclusive sums
-    const uint32_t lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const V y = __shfl_up(x, d);
-        if (lane >= (uint32_t)d) x += y;
-    }
-    return x;
-}
 // Exclusive sum over the threads, and the total. The scratch array is free again after the next barrier.
 template <class V>
 __device__ __forceinline__ V block_before(V x, V* scratch, V* total) {
@@ -197,7 +183,7 @@ __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t 
                 s += w[i];
             }
             uint32_t c_before = wave_upto(c) - c;
-            uint64_t s_before = wave_upto((unsigned long long)s) - s;
+            uint64_t s_before = wave_upto(s) - s;
             const uint64_t reached = __ballot(c_before + c >= need_count || s_before + s >= need_weight);
             const uint32_t at = reached ? (uint32_t)__ffsll((unsigned long long)reached) - 1 : 63u;
             if (lane == at) {
@@ -298,9 +284,9 @@ __device__ __forceinline__ void draw_from_row(const T* logits, uint32_t vocab, f
         if (o == cut.order) ++ties, tie_weight = scale.weight(l, top);
         else above += scale.weight(l, top);
     }
-    ties = __shfl(wave_upto(ties), 63);
-    tie_weight = (uint32_t)wave_max(tie_weight);
-    above = __shfl(wave_upto((unsigned long long)above), 63);
+    ties = wave_sum(ties);
+    tie_weight = wave_max(tie_weight, 0u);
+    above = wave_sum(above);
     __syncthreads();
     if (lane == 0) sh.wave32[wave] = ties;
     __syncthreads();
@@ -329,13 +315,13 @@ __device__ __forceinline__ void draw_from_row(const T* logits, uint32_t vocab, f
             const uint64_t tie_lanes = __ballot(tie);
             if (tie && (uint32_t)__popcll(tie_lanes & ((1ull << lane) - 1)) >= ties_left) w = 0;
             ties_left -= min(ties_left, (uint32_t)__popcll(tie_lanes));
-            const uint64_t upto = wave_upto((unsigned long long)w);
+            const uint64_t upto = wave_upto((uint64_t)w);
             const uint64_t found = __ballot(before + upto > target);
             if (found) {
                 if (lane == 0) sh.token = i0 + (uint32_t)__ffsll((unsigned long long)found) - 1;
                 break;
             }
-            before += __shfl((unsigned long long)upto, 63);
+            before += from_lane(upto, 63);
         }
     }
     __syncthreads();
@@ -389,11 +375,8 @@ __device__ __forceinline__ uint32_t draw_from_chunk(const T* logits, uint32_t vo
             last = from + j;
         }
     }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        first = min(first, (uint32_t)__shfl_xor(first, d));
-        last = max(last, (uint32_t)__shfl_xor(last, d));
-    }
+    first = wave_min(first, kAll);
+    last = wave_max(last, 0u);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.wave32[threadIdx.x >> 6] = first, sh.wave64[threadIdx.x >> 6] = last;
     __syncthreads();
@@ -462,12 +445,9 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
         for (int j = 0; j < 8; ++j) high = fmaxf(high, l[v][j]);
     // the best logit, and the mean of the threads' best ones: few logits of a chunk lie above that
     float chunk_top = high, mean = high > -INFINITY ? high : 0.0f, some = high > -INFINITY ? 1.0f : 0.0f;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        chunk_top = fmaxf(chunk_top, __shfl_xor(chunk_top, d));
-        mean += __shfl_xor(mean, d);
-        some += __shfl_xor(some, d);
-    }
+    chunk_top = wave_max(chunk_top, -INFINITY);
+    mean = wave_sum(mean);
+    some = wave_sum(some);
     if (lane == 0) sh.wave_float[wave] = chunk_top, sh.wave_mean[wave] = mean, sh.wave32[wave] = (uint32_t)some;
     __syncthreads();
     mean = 0.0f, some = 0.0f;
@@ -486,8 +466,7 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (l[v][j] == chunk_top) best_at = min(best_at, begin + 8 * (v * kThreads + threadIdx.x) + j);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) best_at = min(best_at, (uint32_t)__shfl_xor(best_at, d));
+    best_at = wave_min(best_at, kAll);
     __syncthreads();
     if (lane == 0) sh.wave32[wave] = best_at;
 
@@ -508,9 +487,7 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
                 if (binned && down < kBins)
                     atomicAdd((unsigned long long*)&sh.bins[down], 1ull << kCountShift | scale.weight_of(e, x == chunk_top));
             }
-        sum = (double)mine * 0x1p-32;
-#pragma unroll
-        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+        sum = wave_sum((double)mine * 0x1p-32);
         if (lane == 0) sh.wave_sum[wave] = sum;
     } else if (!greedy && filtered) {
         // few of a wave's logits exceed the mean: they are marked first and then taken together
@@ -546,7 +523,7 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
             uint32_t upto = wave_upto(n) - n;
 #pragma unroll
             for (int i = 0; i < kBins / 64; ++i) fit += (upto += (uint32_t)(sh.bins[kBins / 64 * lane + i] >> kCountShift)) <= rows.room;
-            fit = __shfl(wave_upto(fit), 63);
+            fit = wave_sum(fit);
             if (lane == 0) sh.digit = summed || mean == -INFINITY ? fit : min(fit, (uint32_t)max(0, min(top_bin - scale.bin(mean), kBins)));
         }
         __syncthreads();
@@ -567,8 +544,7 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
             }
             marks[v * kThreads + threadIdx.x] = (uint8_t)mark;
         }
-#pragma unroll
-        for (int d = 32; d; d >>= 1) outside = fmaxf(outside, __shfl_xor(outside, d));
+        outside = wave_max(outside, -INFINITY);
         if (lane == 0) sh.wave_float[wave] = outside;
         __syncthreads();
 #pragma unroll
@@ -605,7 +581,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
     const uint64_t tail = mine && filtered ? record[threadIdx.x * words + 2] : (uint64_t)__float_as_uint(-INFINITY);
     const double sum = mine && set.summed ? __builtin_bit_cast(double, record[threadIdx.x * words + 1]) : 0.0;
     const uint64_t own = best;
-    best = wave_max(best);
+    best = wave_max(best, (uint64_t)0);
     if (lane == 0) sh.wave64[wave] = best;
     __syncthreads();
 #pragma unroll
@@ -621,8 +597,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
         return;
     }
     float outside = __uint_as_float((uint32_t)tail);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) outside = fmaxf(outside, __shfl_xor(outside, d));
+    outside = wave_max(outside, -INFINITY);
     if (lane == 0) sh.wave_float[wave] = outside;
     if (mine) sh.tops[threadIdx.x] = logit_of((uint32_t)(own >> 32)), sh.sums[threadIdx.x] = sum, sh.held[threadIdx.x] = (uint32_t)(tail >> 32);
     __syncthreads();
@@ -797,11 +772,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
                 weight[i] = in ? scale.weight(v, top) : 0;
                 if (weight[i]) lowest = min(lowest, order[i]), highest = max(highest, order[i]);
             }
-#pragma unroll
-            for (int d = 32; d; d >>= 1) {
-                lowest = min(lowest, (uint32_t)__shfl_xor(lowest, d));
-                highest = max(highest, (uint32_t)__shfl_xor(highest, d));
-            }
+            lowest = wave_min(lowest, kAll);
+            highest = wave_max(highest, 0u);
             if (lane == 0) sh.wave32[wave] = lowest, sh.wave64[wave] = highest;
             __syncthreads();
 #pragma unroll
@@ -833,8 +805,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
                     if (b + (int)lane < above) x += (double)(w & kWeight);
                 }
                 x *= sh.unit[c];
-#pragma unroll
-                for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+                x = wave_sum(x);
                 if (lane == 0) sh.sums[c] = x;
             }
             __syncthreads();
@@ -867,9 +838,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
                 if (weight[i] && order[i] == cut.order && tie++ >= cut.ties) weight[i] = 0;
                 thread_sum += weight[i];
             }
-            unsigned long long kept_sum;
-            uint64_t before = block_before((unsigned long long)thread_sum, (unsigned long long*)sh.wave64, &kept_sum);
-            sum64 = kept_sum;
+            uint64_t before = block_before(thread_sum, sh.wave64, &sum64);
             const uint64_t target = min(share(sum64, a.uniform[r], false), sum64 - 1);
             if (target >= before && target < before + thread_sum) {
 #pragma unroll
