@@ -439,7 +439,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
 // ---------------------------------------------------------------------------------
 // Many rows
 // ---------------------------------------------------------------------------------
-// One workgroup: 8 waves of 32 rows of one sequence and KV head against the keys that they see, 64 at a time through
+// One workgroup: 8 (or 4) waves of 32 rows of one sequence and KV head against the keys that they see, 64 at a time through
 // LDS. Products are taken transposed, S^T = K Q^T and O^T = V^T P^T (32 x 32 x 16), so that a lane holds scores of
 // one row only and the P that it computed is already the second product's operand: key slots are permuted alike in P
 // and V^T, which a sum over keys allows. V^T comes out of LDS by transposing reads.
@@ -453,7 +453,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
 // attention_join_kernel.
 template <int D>
 struct Tile {
-    static constexpr int kWaves = D == 256 ? 4 : 8;           // D = 256: twice the registers a row
+    // D = 256 needs twice the registers a row; D = 64 has fewer products to a score, and two workgroups of 4 waves on a
+    // compute unit overlap better than one of 8 (4096 tokens over 4096 keys, 16 heads: 82 and 102 us; D = 128, 4096
+    // over 32768: 2.37 and 2.14 ms).
+    static constexpr int kWaves = D == 128 ? 8 : 4;
+    static constexpr uint32_t kFill = D == 64 ? 512 : 256;    // workgroups that run at once
     static constexpr int kRows = 32 * kWaves;
     static constexpr int kKeys = D == 256 ? 32 : 64;
     static constexpr int kChunks = D / 8;                     // 16-byte chunks of a row
@@ -476,7 +480,6 @@ struct TilePlan {
                            // rows of D sums and then their m and l
     uint64_t bytes;
 };
-constexpr uint32_t kTileFill = 256;    // workgroups that run at once: one a compute unit
 constexpr uint64_t kPartsAt = 256;
 constexpr uint32_t kLeastChunk = 8;    // steps: a split's part of the sums costs as much as one
 
@@ -487,9 +490,9 @@ __host__ __device__ inline uint64_t most_steps(uint64_t keys, uint64_t unit, uin
 }
 
 // The tiles of all sequences and their splits. Only the device knows the lengths, so every wave reads them, 64 sequences
-// at a time. `chunk`, the steps of a split, is the least that makes no more than kTileFill workgroups: a second round
+// at a time. `chunk`, the steps of a split, is the least that makes no more workgroups than run at once: a second round
 // for a few of them costs more than it shortens the first, and so do parts of sums for tiles that fill the card by
-// themselves (4096 tokens over 4096 keys, 16 heads of 64: 103 us whole, 143 us split into 512).
+// themselves (4096 tokens over 4096 keys, 16 heads of 64, 256 tiles: 103 us whole, 143 us split into 512).
 template <int D>
 struct TileWork {
     typedef Tile<D> C;
@@ -517,16 +520,16 @@ struct TileWork {
         tiles = wave_sum(tiles) * a.kv_heads;
         longest = wave_max(longest, 0u);
         chunk = max(longest, 1u);
-        if (plan.splits == 1 || 2 * tiles > kTileFill) return;
-        // fewer than 2^8 tiles of fewer than 2^24 steps
-        chunk = max(max((wave_sum(total) * a.kv_heads + kTileFill - 1) / kTileFill, (longest + plan.splits - 1) / plan.splits), kLeastChunk);
-        for (;;) {   // twice the even share makes at most kTileFill / 2 + tiles
+        if (plan.splits == 1 || 2 * tiles > C::kFill) return;
+        // no more than 2^8 tiles of fewer than 2^24 steps
+        chunk = max(max((wave_sum(total) * a.kv_heads + C::kFill - 1) / C::kFill, (longest + plan.splits - 1) / plan.splits), kLeastChunk);
+        for (;;) {   // twice the even share makes at most C::kFill / 2 + tiles
             uint32_t items = 0;
             for (int s0 = 0; s0 < (int)a.sequences; s0 += 64) {
                 if (a.sequences > 64) n = tiles_of(a, s0 + lane, &steps);
                 items += n * ((steps + chunk - 1) / chunk);
             }
-            if (wave_sum(items) * a.kv_heads <= kTileFill || chunk >= longest) break;
+            if (wave_sum(items) * a.kv_heads <= C::kFill || chunk >= longest) break;
             chunk += chunk / 8 + 1;
         }
     }
@@ -558,7 +561,7 @@ typedef __attribute__((address_space(3))) char* lds_bytes;
 typedef const __attribute__((address_space(1))) void* global_void;
 
 template <class T, int D, bool Large>
-__global__ __launch_bounds__(64 * Tile<D>::kWaves) void attention_tile_kernel(const ls_hip_attention a, uint32_t shift,
+__global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attention_tile_kernel(const ls_hip_attention a, uint32_t shift,
                                                                               const TilePlan plan) {
     typedef Tile<D> C;
     constexpr int kKeys = C::kKeys, kSub = kKeys / 32;
@@ -931,21 +934,24 @@ SplitPlan plan_rows(const ls_hip_attention& a) {
 }
 
 // Room for the splits of the tiles, as if all tokens belonged to few chunks.
-TilePlan plan_tiles(const ls_hip_attention& a, uint64_t tile_rows, uint64_t tile_keys, uint64_t offset) {
+template <int D>
+TilePlan plan_tiles(const ls_hip_attention& a, uint64_t offset) {
+    typedef Tile<D> C;
     TilePlan p{};
     const uint64_t group = a.q_heads / a.kv_heads;
-    const uint64_t least = std::max<uint64_t>(1, a.tokens * group / tile_rows) * a.kv_heads;   // workgroups without splits
-    const uint64_t steps = most_steps(a.max_context, tile_keys, tile_rows / group + 2, a.window, a.sinks);
-    p.splits = (uint32_t)std::max<uint64_t>(1, std::min(kTileFill / least, (steps + kLeastChunk - 1) / kLeastChunk));
+    const uint64_t least = std::max<uint64_t>(1, a.tokens * group / C::kRows) * a.kv_heads;   // workgroups without splits
+    const uint64_t steps = most_steps(a.max_context, C::kKeys, C::kRows / group + 2, a.window, a.sinks);
+    p.splits = (uint32_t)std::max<uint64_t>(1, std::min(C::kFill / least, (steps + kLeastChunk - 1) / kLeastChunk));
     p.offset = (offset + 255) / 256 * 256;
     if (p.splits > 1) p.bytes = p.offset + kPartsAt + p.splits * (uint64_t)a.tokens * a.q_heads * (a.head_dim + 2) * sizeof(float);
     return p;
 }
 // Workgroups of the tiles: every tile ends with a split that is not full.
-uint32_t tile_grid(const ls_hip_attention& a, uint64_t tile_rows) {
+template <int D>
+uint32_t tile_grid(const ls_hip_attention& a) {
     const uint64_t rows = (uint64_t)a.tokens * (a.q_heads / a.kv_heads);
-    const uint64_t tiles = rows / tile_rows + std::min<uint64_t>(a.sequences, rows / (kRows + 1));
-    return (uint32_t)((tiles + kTileFill / a.kv_heads + 1) * a.kv_heads);
+    const uint64_t tiles = rows / Tile<D>::kRows + std::min<uint64_t>(a.sequences, rows / (kRows + 1));
+    return (uint32_t)((tiles + Tile<D>::kFill / a.kv_heads + 1) * a.kv_heads);
 }
 
 struct Plan {
@@ -961,8 +967,9 @@ Plan make_plan(const ls_hip_attention& a) {
     p.by_tiles = (uint64_t)a.max_new * group > (uint64_t)kRows;
     if (p.by_rows) p.rows = plan_rows(a);
     if (p.by_tiles)
-        p.tiles = a.head_dim == 256 ? plan_tiles(a, Tile<256>::kRows, Tile<256>::kKeys, p.rows.bytes)
-                                    : plan_tiles(a, Tile<128>::kRows, Tile<128>::kKeys, p.rows.bytes);
+        p.tiles = a.head_dim == 64    ? plan_tiles<64>(a, p.rows.bytes)
+                  : a.head_dim == 128 ? plan_tiles<128>(a, p.rows.bytes)
+                                      : plan_tiles<256>(a, p.rows.bytes);
     p.bytes = std::max(p.rows.bytes, p.tiles.bytes);
     return p;
 }
@@ -977,7 +984,7 @@ void launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
     }
     if (plan.by_tiles) {
         typedef Tile<D> C;
-        const uint32_t grid = tile_grid(a, C::kRows);
+        const uint32_t grid = tile_grid<D>(a);
         if (a.page_size >= 16) attention_tile_kernel<T, D, true><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
         else attention_tile_kernel<T, D, false><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
         if (plan.tiles.splits > 1)
