@@ -5,6 +5,7 @@
 #include <hip/hip_fp16.h>
 #include <cerrno>
 #include <cmath>
+#include <type_traits>
 #include "leanstream_hip.h"
 #include "wave_ops.h"
 
@@ -88,6 +89,18 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(const ls_hip_block
     if (gate)
 #pragma unroll
         for (int v = 0; v < Vecs; ++v) gt[v] = load8(gate, lane + v * kLanes, width);
+    // Rows of few registers hold the weights too, so that one row waits for memory once; many long rows find them in
+    // the caches, and the registers are better spent on more waves.
+    constexpr bool kEarly = Vecs <= 2;
+    typename Vec8<T>::type before[kEarly ? Vecs : 1] = {}, after[kEarly ? Vecs : 1] = {};
+    if constexpr (kEarly) {
+        if (post)
+#pragma unroll
+            for (int v = 0; v < Vecs; ++v) before[v] = load8(post, lane + v * kLanes, width);
+        if (a.normed)
+#pragma unroll
+            for (int v = 0; v < Vecs; ++v) after[v] = load8(pre, lane + v * kLanes, width);
+    }
 
     float inv = 1.0f;
     if (post) {
@@ -102,7 +115,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(const ls_hip_block
 #pragma unroll
     for (int v = 0; v < Vecs; ++v) {
         typename Vec8<T>::type w = {};
-        if (post) w = load8(post, lane + v * kLanes, width);
+        if (post) w = kEarly ? before[kEarly ? v : 0] : load8(post, lane + v * kLanes, width);
         const bool in = 8 * (lane + v * kLanes) < width;   // beyond the end 0 * inv may be NaN
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -120,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(const ls_hip_block
     inv = 1.0f / sqrtf(row_sum<Waves>(sum, scratch) / n + a.eps);
 #pragma unroll
     for (int v = 0; v < Vecs; ++v) {
-        const typename Vec8<T>::type w = load8(pre, lane + v * kLanes, width);
+        const typename Vec8<T>::type w = kEarly ? after[kEarly ? v : 0] : load8(pre, lane + v * kLanes, width);
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = h[v][j] * inv * (a.weight_offset + to_float(w[j]));
@@ -138,111 +151,115 @@ void launch_norm(const ls_hip_block_norm& a, hipStream_t st) {
     else block_norm_kernel<T, 4, 8><<<a.rows, kThreads, 0, st>>>(a);
 }
 
-// The sequence that holds row t of q: the last one that starts at or before it, 64 candidates at a time.
-__device__ __forceinline__ int find_sequence(const int32_t* q_start, uint32_t sequences, int t) {
-    const uint32_t lane = threadIdx.x & 63;
-    int found = 0;
-    for (uint32_t s0 = 0; s0 < sequences; s0 += 64) {
-        const uint64_t at = __ballot(s0 + lane < sequences && q_start[min(s0 + lane, sequences - 1)] <= t);
-        if (!at) break;
-        found = (int)s0 + 63 - __clzll((long long)at);
-    }
-    return found;
-}
+// Lengths and page tables do not change while a kernel runs: uniform ones come over the scalar cache.
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef const __attribute__((address_space(4))) int32_t* Table;
+#else
+typedef const int32_t* Table;
+#endif
 
 // One workgroup a token: its q and k heads are rotated and its k and v put into the slot of its position.
-// Bound by memory (and by the latency of q_start -> context -> page for few tokens). Chunks of 8 dimensions go
-// in 16-byte words where the head and the rotated part divide into them (Wide); otherwise pairs go alone.
+// Bound by memory, for few tokens by the latency of q_start -> context -> page -> tables: a thread's first values are
+// loaded before. Chunks of 8 dimensions go in 16-byte words where the head and the rotated part divide into them
+// (Wide); otherwise dimensions go alone.
+// Threads of a token: up to a token a compute unit the wait for its first values counts (32 tokens: 5.4 us with 512, 6.0
+// with 256), beyond it the workgroups under way (8192 tokens: 81 and 70 us).
+constexpr uint32_t kAppendThreads = 512, kAppendFew = 256;
 template <class T, bool Wide>
-__global__ __launch_bounds__(kThreads) void append_kernel(const ls_hip_append a, uint32_t page_shift) {
-    const int64_t t = blockIdx.x;
-    const int s = find_sequence(a.q_start, a.sequences, (int)t);
-    const int first = a.q_start[s], end = a.q_start[s + 1];
-    if (t < first || t >= end) return;   // no sequence's token
-    const int64_t pos = (int64_t)a.context[s] - (end - t);
-    if (pos < 0 || (a.rot && pos >= (int64_t)a.positions) || (pos >> page_shift) >= (int64_t)a.table_width) {
-        if (threadIdx.x == 0 && a.status) atomicOr(a.status, (uint32_t)LS_STATUS_RANGE);
-        return;
-    }
-    const int page = a.page_table[s * a.table_stride + (pos >> page_shift)];
-    const int64_t slot = pos & ((1 << page_shift) - 1);
-    if ((uint32_t)page >= a.pages) {
-        if (threadIdx.x == 0 && a.status) atomicOr(a.status, (uint32_t)LS_STATUS_BAD_DESCRIPTOR);
-        return;
-    }
-    // units of a head: rotated ones (a pair of chunks, or of dimensions), then copied ones
-    constexpr uint32_t kUnit = Wide ? 8 : 1;
-    const uint32_t half = a.rot / 2;
-    const uint32_t turned = a.interleaved && Wide ? a.rot / 8 : half / kUnit;
-    const uint32_t plain = (a.head_dim - a.rot) / kUnit;
-    const uint32_t turn_units = (a.q_heads + a.kv_heads) * turned, plain_units = (a.q_heads + a.kv_heads) * plain;
-    const uint32_t v_units = a.kv_heads * (a.head_dim / kUnit);
-    const float* cosine = a.cos + pos * half;
-    const float* sine = a.sin + pos * half;
-    auto place = [&](uint32_t head, const T*& src, T*& dst) {
-        if (head < a.q_heads) {
-            src = (const T*)a.q + t * a.q_token_stride + head * a.q_head_stride;
-            dst = (T*)a.q_out + t * a.q_out_token_stride + head * a.q_out_head_stride;
-        } else {
-            head -= a.q_heads;
-            src = (const T*)a.k + t * a.k_token_stride + head * a.k_head_stride;
-            dst = (T*)a.k_pages + page * a.k_page_stride + head * a.k_head_page_stride + slot * a.k_slot_stride;
-        }
-    };
+__global__ __launch_bounds__(kAppendThreads) void append_kernel(const ls_hip_append a, uint32_t page_shift) {
     typedef typename Vec8<T>::type vec8;
     typedef typename Vec8<float>::half float4u;
-    for (uint32_t i = threadIdx.x; i < turn_units; i += kThreads) {
-        const uint32_t head = i / turned, u = i % turned;
-        const T* src;
-        T* dst;
-        place(head, src, dst);
+    typedef std::conditional_t<Wide, vec8, T> Piece;
+    const int64_t t = blockIdx.x;
+    const uint32_t lane = threadIdx.x & 63;
+    const int start = a.q_start[min(lane, a.sequences - 1)];   // of the first 64 sequences
+
+    // Units of a token: rotated ones (q heads, then k heads), copied ones of q and k, then v. A rotated unit is a pair
+    // of pieces, or with interleaved pairs in 16-byte words one piece.
+    constexpr uint32_t kUnit = Wide ? 8 : 1;
+    const uint32_t half = a.rot / 2, heads = a.q_heads + a.kv_heads;
+    const bool lone = a.interleaved && Wide;
+    const uint32_t turned = lone ? a.rot / 8 : half / kUnit, plain = (a.head_dim - a.rot) / kUnit, whole = a.head_dim / kUnit;
+    const uint32_t turn_units = heads * turned, plain_units = turn_units + heads * plain, units = plain_units + a.kv_heads * whole;
+    int64_t pos = -1, slot = 0;
+    int page = 0;
+    for (uint32_t i0 = 0; i0 < units; i0 += blockDim.x) {
+        const uint32_t i = min(i0 + threadIdx.x, units - 1);   // beyond the end: loaded only
+        const bool turn = i < turn_units, value = i >= plain_units;
+        const uint32_t j = turn ? i : value ? i - plain_units : i - turn_units, each = turn ? turned : value ? whole : plain;
+        const uint32_t head = j / each, u = j % each;
+        const bool query = !value && head < a.q_heads;
+        const uint32_t kv = value || query ? head : head - a.q_heads;
+        const T* src = value   ? (const T*)a.v + t * a.v_token_stride + kv * a.v_head_stride
+                       : query ? (const T*)a.q + t * a.q_token_stride + kv * a.q_head_stride
+                               : (const T*)a.k + t * a.k_token_stride + kv * a.k_head_stride;
+        uint32_t x = kUnit * u + (turn || value ? 0 : a.rot), y = x + half;   // the dimensions of its pieces
+        if (turn && !Wide && a.interleaved) x = 2 * u, y = 2 * u + 1;
+        const Piece p = *(const Piece*)(src + x);
+        Piece q = p;
+        if (turn && !lone) q = *(const Piece*)(src + y);
+
+        if (pos < 0) {   // once: the sequence (the last one that starts at or before t), its length, the page
+            int s = 0;
+            for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
+                const int first = s0 ? a.q_start[min(s0 + lane, a.sequences - 1)] : start;
+                const uint32_t count = __popcll(__ballot(s0 + lane < a.sequences && first <= t));
+                if (!count) break;
+                s = (int)(s0 + count) - 1;
+            }
+            s = __builtin_amdgcn_readfirstlane(s);
+            const int first = ((Table)a.q_start)[s], end = ((Table)a.q_start)[s + 1];
+            if (t < first || t >= end) return;   // no sequence's token
+            pos = (int64_t)((Table)a.context)[s] - (end - t);
+            if (pos < 0 || (a.rot && pos >= (int64_t)a.positions) || (pos >> page_shift) >= (int64_t)a.table_width) {
+                if (threadIdx.x == 0 && a.status) atomicOr(a.status, (uint32_t)LS_STATUS_RANGE);
+                return;
+            }
+            page = ((Table)a.page_table)[s * a.table_stride + (pos >> page_shift)];
+            slot = pos & ((1 << page_shift) - 1);
+            if ((uint32_t)page >= a.pages) {
+                if (threadIdx.x == 0 && a.status) atomicOr(a.status, (uint32_t)LS_STATUS_BAD_DESCRIPTOR);
+                return;
+            }
+        }
+        if (i0 + threadIdx.x >= units) return;
+        T* dst = value   ? (T*)a.v_pages + page * a.v_page_stride + kv * a.v_head_page_stride + slot * a.v_slot_stride
+                 : query ? (T*)a.q_out + t * a.q_out_token_stride + kv * a.q_out_head_stride
+                         : (T*)a.k_pages + page * a.k_page_stride + kv * a.k_head_page_stride + slot * a.k_slot_stride;
+        if (!turn) {
+            *(Piece*)(dst + x) = p;
+            continue;
+        }
+        const float* cosine = a.cos + pos * half;
+        const float* sine = a.sin + pos * half;
         if constexpr (!Wide) {
-            const uint32_t x = a.interleaved ? 2 * u : u, y = a.interleaved ? 2 * u + 1 : u + half;
-            const float c = cosine[u], sn = sine[u], p = to_float(src[x]), q = to_float(src[y]);
-            dst[x] = (T)(p * c - q * sn);
-            dst[y] = (T)(q * c + p * sn);
-        } else if (a.interleaved) {   // four pairs
-            const vec8 p = *(const vec8*)(src + 8 * u);
+            const float c = cosine[u], sn = sine[u], v = to_float(p), w = to_float(q);
+            dst[x] = (T)(v * c - w * sn);
+            dst[y] = (T)(w * c + v * sn);
+        } else if (lone) {   // four pairs
             const float4u c = *(const float4u*)(cosine + 4 * u), sn = *(const float4u*)(sine + 4 * u);
             vec8 r;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float x = to_float(p[2 * j]), y = to_float(p[2 * j + 1]);
-                r[2 * j] = (T)(x * c[j] - y * sn[j]);
-                r[2 * j + 1] = (T)(y * c[j] + x * sn[j]);
+            for (int k = 0; k < 4; ++k) {
+                const float v = to_float(p[2 * k]), w = to_float(p[2 * k + 1]);
+                r[2 * k] = (T)(v * c[k] - w * sn[k]);
+                r[2 * k + 1] = (T)(w * c[k] + v * sn[k]);
             }
-            *(vec8*)(dst + 8 * u) = r;
+            *(vec8*)(dst + x) = r;
         } else {   // eight pairs
-            const vec8 p = *(const vec8*)(src + 8 * u), q = *(const vec8*)(src + half + 8 * u);
-            const float4u c0 = *(const float4u*)(cosine + 8 * u), c1 = *(const float4u*)(cosine + 8 * u + 4);
-            const float4u s0 = *(const float4u*)(sine + 8 * u), s1 = *(const float4u*)(sine + 8 * u + 4);
-            vec8 r, w;
+            const float4u c0 = *(const float4u*)(cosine + x), c1 = *(const float4u*)(cosine + x + 4);
+            const float4u s0 = *(const float4u*)(sine + x), s1 = *(const float4u*)(sine + x + 4);
+            vec8 r, r2;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = to_float(p[j]), y = to_float(q[j]), c = j < 4 ? c0[j % 4] : c1[j % 4],
-                            sn = j < 4 ? s0[j % 4] : s1[j % 4];
-                r[j] = (T)(x * c - y * sn);
-                w[j] = (T)(y * c + x * sn);
+            for (int k = 0; k < 8; ++k) {
+                const float v = to_float(p[k]), w = to_float(q[k]), c = k < 4 ? c0[k % 4] : c1[k % 4],
+                            sn = k < 4 ? s0[k % 4] : s1[k % 4];
+                r[k] = (T)(v * c - w * sn);
+                r2[k] = (T)(w * c + v * sn);
             }
-            *(vec8*)(dst + 8 * u) = r;
-            *(vec8*)(dst + half + 8 * u) = w;
+            *(vec8*)(dst + x) = r;
+            *(vec8*)(dst + y) = r2;
         }
-    }
-    for (uint32_t i = threadIdx.x; i < plain_units + v_units; i += kThreads) {
-        const T* src;
-        T* dst;
-        uint32_t at;
-        if (i < plain_units) {
-            place(i / plain, src, dst);
-            at = a.rot + kUnit * (i % plain);
-        } else {
-            const uint32_t each = a.head_dim / kUnit, head = (i - plain_units) / each;
-            src = (const T*)a.v + t * a.v_token_stride + head * a.v_head_stride;
-            dst = (T*)a.v_pages + page * a.v_page_stride + head * a.v_head_page_stride + slot * a.v_slot_stride;
-            at = kUnit * ((i - plain_units) % each);
-        }
-        if constexpr (Wide) *(vec8*)(dst + at) = *(const vec8*)(src + at);
-        else dst[at] = src[at];
     }
 }
 
@@ -311,6 +328,6 @@ extern "C" int ls_hip_append_enqueue(const ls_hip_append* a, void* stream) {
     const bool wide = a->head_dim % 8 == 0 && a->rot % (a->interleaved ? 8 : 16) == 0;
     const auto kernel = a->dtype == LS_TYPE_F16 ? wide ? append_kernel<_Float16, true> : append_kernel<_Float16, false>
                                                 : wide ? append_kernel<__bf16, true> : append_kernel<__bf16, false>;
-    kernel<<<a->tokens, kThreads, 0, st>>>(*a, shift);
+    kernel<<<a->tokens, a->tokens <= kAppendFew ? kAppendThreads : kAppendThreads / 2, 0, st>>>(*a, shift);
     return finish();
 }
