@@ -164,9 +164,10 @@ typedef const int32_t* Table;
 // (Wide); otherwise dimensions go alone.
 // Threads of a token: up to a token a compute unit the wait for its first values counts (32 tokens: 5.4 us with 512, 6.0
 // with 256), beyond it the workgroups under way (8192 tokens: 81 and 70 us).
-constexpr uint32_t kAppendThreads = 512, kAppendFew = 256;
-template <class T, bool Wide>
-__global__ __launch_bounds__(kAppendThreads) void append_kernel(const ls_hip_append a, uint32_t page_shift) {
+constexpr uint32_t kAppendThreads = 512;
+constexpr uint32_t kAppendFew = 256;
+template <class T, bool Wide, uint32_t Threads>
+__global__ __launch_bounds__(Threads) void append_kernel(const ls_hip_append a, uint32_t page_shift) {
     typedef typename Vec8<T>::type vec8;
     typedef typename Vec8<float>::half float4u;
     typedef std::conditional_t<Wide, vec8, T> Piece;
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(const ls_hip_app
     const uint32_t turn_units = heads * turned, plain_units = turn_units + heads * plain, units = plain_units + a.kv_heads * whole;
     int64_t pos = -1, slot = 0;
     int page = 0;
-    for (uint32_t i0 = 0; i0 < units; i0 += blockDim.x) {
+    for (uint32_t i0 = 0; i0 < units; i0 += Threads) {
         const uint32_t i = min(i0 + threadIdx.x, units - 1);   // beyond the end: loaded only
         const bool turn = i < turn_units, value = i >= plain_units;
         const uint32_t j = turn ? i : value ? i - plain_units : i - turn_units, each = turn ? turned : value ? whole : plain;
@@ -326,8 +327,13 @@ extern "C" int ls_hip_append_enqueue(const ls_hip_append* a, void* stream) {
     const auto st = static_cast<hipStream_t>(stream);
     const uint32_t shift = __builtin_ctz(a->page_size);
     const bool wide = a->head_dim % 8 == 0 && a->rot % (a->interleaved ? 8 : 16) == 0;
-    const auto kernel = a->dtype == LS_TYPE_F16 ? wide ? append_kernel<_Float16, true> : append_kernel<_Float16, false>
-                                                : wide ? append_kernel<__bf16, true> : append_kernel<__bf16, false>;
-    kernel<<<a->tokens, a->tokens <= kAppendFew ? kAppendThreads : kAppendThreads / 2, 0, st>>>(*a, shift);
+    const auto launch = [&](auto threads) {
+        constexpr uint32_t n = decltype(threads)::value;
+        const auto kernel = a->dtype == LS_TYPE_F16 ? wide ? append_kernel<_Float16, true, n> : append_kernel<_Float16, false, n>
+                                                    : wide ? append_kernel<__bf16, true, n> : append_kernel<__bf16, false, n>;
+        kernel<<<a->tokens, n, 0, st>>>(*a, shift);
+    };
+    if (a->tokens <= kAppendFew) launch(std::integral_constant<uint32_t, kAppendThreads>());
+    else launch(std::integral_constant<uint32_t, kAppendThreads / 2>());
     return finish();
 }

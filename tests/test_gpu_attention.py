@@ -328,6 +328,55 @@ def test_wrong_tensors_are_refused(torch_gpu):
     p = Problem(torch, "float16", **CASES["few_tokens"])
     with pytest.raises(RuntimeError, match="Native attention failed: 22"):
         p.on_gpu(max_context=100000).enqueue()
+    long = Problem(torch, "float16", **CASES["decode"])
+    call = long.on_gpu(workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(RuntimeError, match="Native attention failed: 28"):
+        call.enqueue()
     with pytest.raises(ValueError, match="float16"):
         p.q = p.q.float()
         p.on_gpu()
+
+
+def test_one_workspace_for_calls_of_every_shape(torch_gpu):
+    """Calls that follow one another on a stream share a workspace, whatever each leaves in it."""
+    torch = torch_gpu
+    names = ["decode", "ragged", "few_tokens", "chunk", "decode_mqa", "window_sinks", "decode"]
+    problems = [Problem(torch, "float16", **CASES[n]) for n in names]
+    need = max(p.on_gpu().workspace.numel() if p.on_gpu().workspace is not None else 0 for p in problems)
+    shared = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    calls = [p.on_gpu(workspace=shared) for p in problems]
+    for _ in range(2):
+        for c in calls:
+            c.enqueue()
+    for p in problems:
+        p.check()
+
+
+def test_long_split_sequences(torch_gpu):
+    """Many splits of few rows and of tiles: one long sequence alone, and long ones among short ones."""
+    torch = torch_gpu
+    for dim, heads, kv, lengths in ((128, 4, 1, [(1, 20000)]), (64, 2, 2, [(3, 9000), (1, 40)]), (128, 8, 2, [(40, 7000)]),
+                                    (64, 4, 4, [(150, 3000), (1, 5000), (20, 6000)]), (256, 4, 1, [(1, 6000), (30, 5000)])):
+        for window, sinks in ((0, 0), (2500, 9)):
+            log("case:", dim, heads, lengths, window)
+            p = Problem(torch, "float16", dim, heads, kv, 32, lengths, window=window, sinks=sinks)
+            p.on_gpu().enqueue()
+            p.check()
+
+
+def test_values_that_are_not_finite_in_split_tiles(torch_gpu):
+    """As above, where the last tile's keys are a split of their own."""
+    torch = torch_gpu
+    p = Problem(torch, "float16", 128, 8, 2, 16, [(40, 3000)])
+    at, slot = int(p.table[0, 2990 // 16]), 2990 % 16
+    p.v[at, 1, slot, 5] = math.inf       # seen by the last 10 tokens, by heads 4 .. 7
+    p.on_gpu().enqueue()
+    torch.cuda.synchronize()
+    got = p.out.cpu().double()
+    assert (got[30:, 4:, 5] == math.inf).all()
+    got[30:, 4:, 5] = 0
+    p.v[at, 1, slot, 5] = 0
+    out, _, tol = p.expected()
+    out[30:, 4:, 5] = 0
+    # that value's weight (below 1 / 100 of a row here) is not missed elsewhere
+    assert ((got - out).abs() <= tol).all()
