@@ -920,14 +920,19 @@ int check(const ls_hip_attention& a) {
     return 0;
 }
 
-// Splits of the sequences that take the row kernel: enough workgroups to fill the card, none with less than a
-// step for each of its waves. Where there are kFill groups already, there is one split.
+// Splits of the sequences that take the row kernel. Long ones make kFill workgroups (131072 keys, 16 groups: 144 us; with
+// half or twice as many 150 and 154). Splits of few steps pay only up to a workgroup a compute unit (32 sequences of 500
+// keys, 256 groups: whole 15 us, in four 20), and one workgroup joins them all: with s steps, about sqrt(2 s) splits
+// cost least (8000 keys: 21 splits 13 us, 63 splits 18). A split has a step for each of its waves.
 SplitPlan plan_rows(const ls_hip_attention& a) {
     SplitPlan p{};
     p.rows = (uint32_t)std::min<uint64_t>((uint64_t)a.max_new * (a.q_heads / a.kv_heads), kRows);
     const uint64_t steps = most_steps(a.max_context, kStepKeys, kRows, a.window, a.sinks), groups = (uint64_t)a.sequences * a.kv_heads;
-    const uint64_t chunk = std::max<uint64_t>(std::max<uint64_t>(1, (steps * groups + kFill - 1) / kFill), (steps + kMaxSplits - 1) / kMaxSplits);
-    p.chunk = (uint32_t)std::min<uint64_t>((chunk + kRowWaves - 1) / kRowWaves * kRowWaves, 1u << 30);
+    const auto even = [&](uint64_t workgroups) { return (steps * groups + workgroups - 1) / workgroups; };
+    uint64_t chunk = std::max(even(kFill), (steps + kMaxSplits - 1) / kMaxSplits);
+    chunk = std::max(chunk, std::min<uint64_t>(even(kFill / 4), 16));
+    chunk = std::max((chunk + kRowWaves - 1) / kRowWaves, (uint64_t)(std::sqrt((double)steps / 2) / kRowWaves + 0.5));
+    p.chunk = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(chunk, 1) * kRowWaves, 1u << 30);
     p.splits = (uint32_t)std::max<uint64_t>(1, (steps + p.chunk - 1) / p.chunk);
     if (p.splits > 1) p.bytes = kCounterBytes + groups * p.splits * p.rows * (a.head_dim + 2) * sizeof(float);
     return p;
