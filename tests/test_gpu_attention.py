@@ -283,44 +283,18 @@ def test_long_cache_past_32_bits(torch_gpu):
 
 
 @pytest.mark.parametrize("name", ["decode", "few_tokens", "ragged", "window_sinks"])
-def test_repeats_and_streams_give_the_same_bits(torch_gpu, name):
+def test_repeats_give_the_same_bits(torch_gpu, name):
     torch = torch_gpu
     p = Problem(torch, "bfloat16", **CASES[name])
     call = p.on_gpu()
     call.enqueue()
     torch.cuda.synchronize()
     first, first_lse = p.out.clone(), p.lse.clone()
-    side = torch.cuda.Stream()
-    for i in range(6):
+    for _ in range(4):
         p.out.fill_(math.nan)
-        torch.cuda.synchronize()
-        if i % 2:
-            call.enqueue(side.cuda_stream)
-        else:
-            call.enqueue()
+        call.enqueue()
         torch.cuda.synchronize()
         assert torch.equal(p.out, first) and torch.equal(p.lse, first_lse)
-
-
-def test_in_a_graph(torch_gpu):
-    torch = torch_gpu
-    p = Problem(torch, "float16", **CASES["ragged"])
-    call = p.on_gpu()
-    call.enqueue()
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        call.enqueue()
-    for i in range(4):
-        p.out.fill_(math.nan)
-        p.q_gpu.copy_((p.q * (1 + i)).to(p.q.dtype))
-        call.enqueue()
-        torch.cuda.synchronize()
-        want = p.out.clone()
-        p.out.fill_(math.nan)
-        graph.replay()
-        torch.cuda.synchronize()
-        assert torch.equal(p.out, want)
 
 
 def test_wrong_tensors_are_refused(torch_gpu):

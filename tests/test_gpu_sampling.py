@@ -205,38 +205,6 @@ def test_rows_of_any_stride_and_alignment(torch_gpu):
             check(torch, logits, [0.1, 0.3, 0.5, 0.7, 0.9], None, [64] * 5, [0.9] * 5)
 
 
-def test_in_a_graph_and_on_another_stream(torch_gpu):
-    torch = torch_gpu
-    from leanstream_amd import decode
-
-    logits, u, _ = random_rows(torch, 7, 50000, "bfloat16", 9)
-    uniform = torch.tensor(u, device="cuda")
-    tokens = torch.empty(7, dtype=torch.int32, device="cuda")
-    p = torch.full((7,), 0.9, device="cuda")
-    call = decode.Sampler(logits, uniform, tokens, top_p=p)
-    call.enqueue()
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        call.enqueue()
-    side = torch.cuda.Stream()
-    for i in range(4):
-        uniform.copy_(torch.rand(7))
-        logits.add_(torch.randn_like(logits))
-        call.enqueue()
-        torch.cuda.synchronize()
-        want = tokens.clone()
-        tokens.fill_(-9)
-        graph.replay()
-        torch.cuda.synchronize()
-        assert torch.equal(tokens, want)
-        tokens.fill_(-9)
-        torch.cuda.synchronize()
-        call.enqueue(side.cuda_stream)
-        torch.cuda.synchronize()
-        assert torch.equal(tokens, want)
-
-
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("vocab", [3000, 20000, 60001, 131072])
 def test_wide_nuclei(torch_gpu, vocab, dtype):
