@@ -65,8 +65,10 @@ __device__ __forceinline__ float row_sum(float x, float* scratch) {
 }
 
 // Bound by memory: every input is read once, all of a thread's loads are under way before the first sum, and
-// the row stays in registers (fp32) from there on. Rows of up to 2048 columns take one wave (no barriers),
-// four to a workgroup; longer ones the whole workgroup. Vecs: eights of a thread.
+// the row stays in registers (fp32) from there on. 8192 rows of 8192 in bf16 with a gate for every element: 120 us,
+// 5.6 TB/s (through LDS and element by element: 589). One row of 4096: 3 us. Vecs: eights of a thread.
+// Rows of up to 2048 columns take one wave (no barriers), four to a workgroup, longer ones the whole workgroup: 8192
+// rows of 512 8.7 and 34.6 us, of 1024 14.2 and 33.2 (22.4 with registers for 2048), of 2048 27.3 and 34.8.
 template <class T, int Waves, int Vecs>
 __global__ __launch_bounds__(kThreads) void block_norm_kernel(const ls_hip_block_norm a) {
     __shared__ float scratch[Waves];
@@ -145,6 +147,7 @@ template <class T>
 void launch_norm(const ls_hip_block_norm& a, hipStream_t st) {
     const uint32_t w = a.width, packed = (a.rows + kThreads / 64 - 1) / (kThreads / 64);
     if (w <= 512) block_norm_kernel<T, 1, 1><<<packed, kThreads, 0, st>>>(a);
+    else if (w <= 1024) block_norm_kernel<T, 1, 2><<<packed, kThreads, 0, st>>>(a);
     else if (w <= 2048) block_norm_kernel<T, 1, 4><<<packed, kThreads, 0, st>>>(a);
     else if (w <= 4096) block_norm_kernel<T, 4, 2><<<a.rows, kThreads, 0, st>>>(a);
     else if (w <= 8192) block_norm_kernel<T, 4, 4><<<a.rows, kThreads, 0, st>>>(a);
@@ -161,9 +164,9 @@ typedef const int32_t* Table;
 // One workgroup a token: its q and k heads are rotated and its k and v put into the slot of its position.
 // Bound by memory, for few tokens by the latency of q_start -> context -> page -> tables: a thread's first values are
 // loaded before. Chunks of 8 dimensions go in 16-byte words where the head and the rotated part divide into them
-// (Wide); otherwise dimensions go alone.
-// Threads of a token: up to a token a compute unit the wait for its first values counts (32 tokens: 5.4 us with 512, 6.0
-// with 256), beyond it the workgroups under way (8192 tokens: 81 and 70 us).
+// (Wide); otherwise dimensions go alone. 8192 tokens of 64 + 8 + 8 heads of 128: 70 us, 4.8 TB/s (alone: 114).
+// Threads of a token: up to a token a compute unit the wait for its first values counts (32 tokens: 4.1 us with 512,
+// 4.6 with 256), beyond it the workgroups under way (8192 tokens: 81 and 70 us).
 constexpr uint32_t kAppendThreads = 512;
 constexpr uint32_t kAppendFew = 256;
 template <class T, bool Wide, uint32_t Threads>
@@ -180,14 +183,17 @@ __global__ __launch_bounds__(Threads) void append_kernel(const ls_hip_append a, 
     constexpr uint32_t kUnit = Wide ? 8 : 1;
     const uint32_t half = a.rot / 2, heads = a.q_heads + a.kv_heads;
     const bool lone = a.interleaved && Wide;
-    const uint32_t turned = lone ? a.rot / 8 : half / kUnit, plain = (a.head_dim - a.rot) / kUnit, whole = a.head_dim / kUnit;
-    const uint32_t turn_units = heads * turned, plain_units = turn_units + heads * plain, units = plain_units + a.kv_heads * whole;
+    const uint32_t turned = lone ? a.rot / 8 : half / kUnit, plain = (a.head_dim - a.rot) / kUnit;
+    const uint32_t whole = a.head_dim / kUnit;
+    const uint32_t turn_units = heads * turned, plain_units = turn_units + heads * plain;
+    const uint32_t units = plain_units + a.kv_heads * whole;
     int64_t pos = -1, slot = 0;
     int page = 0;
     for (uint32_t i0 = 0; i0 < units; i0 += Threads) {
         const uint32_t i = min(i0 + threadIdx.x, units - 1);   // beyond the end: loaded only
         const bool turn = i < turn_units, value = i >= plain_units;
-        const uint32_t j = turn ? i : value ? i - plain_units : i - turn_units, each = turn ? turned : value ? whole : plain;
+        const uint32_t j = turn ? i : value ? i - plain_units : i - turn_units;
+        const uint32_t each = turn ? turned : value ? whole : plain;
         const uint32_t head = j / each, u = j % each;
         const bool query = !value && head < a.q_heads;
         const uint32_t kv = value || query ? head : head - a.q_heads;
@@ -271,10 +277,12 @@ int check(const ls_hip_block_norm& a) {
     if (!a.width || a.dtype > LS_TYPE_F32 || !(a.eps >= 0.0f && a.eps < INFINITY)) return EINVAL;
     if (!(std::fabs(a.residual_scale) < INFINITY) || !(std::fabs(a.weight_offset) < INFINITY)) return EINVAL;
     const uintptr_t element = a.dtype == LS_TYPE_F32 ? 4 : 2;
-    for (const void* p : {a.block, a.residual, a.gate, a.post_weight, a.pre_weight, (const void*)a.hidden, (const void*)a.normed})
+    for (const void* p : {a.block, a.residual, a.gate, a.post_weight, a.pre_weight, (const void*)a.hidden,
+         (const void*)a.normed})
         if (!aligned(p, element)) return EINVAL;
     if (a.block_stride < 0 || a.residual_stride < 0 || a.gate_stride < 0) return EINVAL;
-    if (a.rows > 1 && ((a.hidden && a.hidden_stride < (int64_t)a.width) || (a.normed && a.normed_stride < (int64_t)a.width)))
+    if (a.rows > 1 && ((a.hidden && a.hidden_stride < (int64_t)a.width) || 
+                       (a.normed && a.normed_stride < (int64_t)a.width)))
         return EINVAL;   // rows of an output must not overlap
     if (a.width > kMaxWidth || a.rows > 0x7fffffffu) return ENOTSUP;
     return 0;
@@ -284,14 +292,16 @@ int check(const ls_hip_append& a) {
     if (!a.k || !a.v || !a.k_pages || !a.v_pages || !a.page_table || !a.q_start || !a.context) return EINVAL;
     if ((a.q_heads && (!a.q || !a.q_out)) || (a.rot && (!a.cos || !a.sin || !a.positions))) return EINVAL;
     if (!a.sequences || !a.kv_heads || !a.head_dim || a.head_dim % 2 || a.rot % 2 || a.rot > a.head_dim) return EINVAL;
-    if (!a.page_size || (a.page_size & (a.page_size - 1)) || !a.pages || !a.table_width || a.dtype > LS_TYPE_F32) return EINVAL;
+    if (!a.page_size || (a.page_size & (a.page_size - 1)) || !a.pages || !a.table_width || a.dtype > LS_TYPE_F32)
+        return EINVAL;
     if (a.tokens > 0x7fffffffu || a.sequences > 0x7fffffffu || a.pages > 0x7fffffffu) return EINVAL;
     if (a.table_stride < 0 || (a.sequences > 1 && a.table_stride < (int64_t)a.table_width)) return EINVAL;
     for (const void* p : {a.q, a.k, a.v, (const void*)a.q_out, (const void*)a.k_pages, (const void*)a.v_pages})
         if (!aligned(p, 2)) return EINVAL;
     const int64_t strides[] = {a.q_token_stride, a.q_head_stride, a.k_token_stride, a.k_head_stride, a.v_token_stride,
                                a.v_head_stride, a.q_out_token_stride, a.q_out_head_stride, a.k_page_stride,
-                               a.k_head_page_stride, a.k_slot_stride, a.v_page_stride, a.v_head_page_stride, a.v_slot_stride};
+                               a.k_head_page_stride, a.k_slot_stride, a.v_page_stride, a.v_head_page_stride,
+                               a.v_slot_stride};
     for (int64_t s : strides)
         if (s < 0) return EINVAL;
     if (a.dtype == LS_TYPE_F32) return ENOTSUP;
@@ -329,8 +339,9 @@ extern "C" int ls_hip_append_enqueue(const ls_hip_append* a, void* stream) {
     const bool wide = a->head_dim % 8 == 0 && a->rot % (a->interleaved ? 8 : 16) == 0;
     const auto launch = [&](auto threads) {
         constexpr uint32_t n = decltype(threads)::value;
-        const auto kernel = a->dtype == LS_TYPE_F16 ? wide ? append_kernel<_Float16, true, n> : append_kernel<_Float16, false, n>
-                                                    : wide ? append_kernel<__bf16, true, n> : append_kernel<__bf16, false, n>;
+        const auto kernel = a->dtype == LS_TYPE_F16
+                                ? wide ? append_kernel<_Float16, true, n> : append_kernel<_Float16, false, n>
+                                : wide ? append_kernel<__bf16, true, n> : append_kernel<__bf16, false, n>;
         kernel<<<a->tokens, n, 0, st>>>(*a, shift);
     };
     if (a->tokens <= kAppendFew) launch(std::integral_constant<uint32_t, kAppendThreads>());
