@@ -44,10 +44,12 @@ struct F16 {
         return __builtin_bit_cast(uint32_t, v2{(_Float16)a, (_Float16)b});
     }
     static __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0,
+                                                      0, 0);
     }
     static __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0,
+                                                      0, 0);
     }
 };
 struct BF16 {
@@ -59,10 +61,12 @@ struct BF16 {
         return __builtin_bit_cast(uint32_t, v2{(__bf16)a, (__bf16)b});
     }
     static __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c,
+                                                       0, 0, 0);
     }
     static __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c,
+                                                       0, 0, 0);
     }
 };
 
@@ -150,11 +154,13 @@ struct Steps {
 // ---------------------------------------------------------------------------------
 // Few rows: one sequence's new tokens times the heads of a group
 // ---------------------------------------------------------------------------------
-// Bound by the bytes of the cache. Keys go 32 at a time from memory straight into matrix operands, with no
-// LDS: a lane of S^T = K Q^T (16 x 16 x 32) holds 16 bytes of one key, and of V a lane loads the same D / 16
-// dimensions of the 8 keys whose P it multiplies, which byte permutes turn into operands. The four waves of a
-// workgroup take the steps of its split in turn and are joined through LDS; the splits of a long sequence are
-// joined by the workgroup that finishes last, in their order.
+// Bound by the bytes of the cache: 4.9 TB/s for 32 sequences of up to 8192 keys (64 / 8 heads of 128, 136 us), 5.5 for
+// two of up to 131072 (145 us); a copy of 2 GiB reaches 4.9. 16-row products waste most of their rows on a single
+// token, at 3 % of what the matrix cores could do. Keys go 32 at a time from memory straight into matrix operands, with
+// no LDS: a lane of S^T = K Q^T (16 x 16 x 32) holds 16 bytes of one key, and of V a lane loads the same D / 16
+// dimensions of the 8 keys whose P it multiplies, which byte permutes turn into operands. The four waves of a workgroup
+// take the steps of its split in turn and are joined through LDS; the splits of a long sequence are joined by the
+// workgroup that finishes last, in their order.
 constexpr int kRowWaves = 4;
 constexpr int kRows = 16;          // sequences of up to this many rows go this way
 constexpr int kStepKeys = 32;
@@ -173,14 +179,16 @@ constexpr uint32_t kFill = 1024;   // workgroups that fill the card, 4 on each o
 constexpr uint64_t kCounterBytes = kFill * sizeof(uint32_t);
 
 __device__ __forceinline__ void store_agent(float* p, float a, float b) {
-    __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, f32x2{a, b}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store((uint64_t*)p, __builtin_bit_cast(uint64_t, f32x2{a, b}), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ f32x2 load_agent(const float* p) {
     return __builtin_bit_cast(f32x2, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
 // The 32 keys of a step: where they lie. Pages of 16 keys and more: both halves lie in one page each, their
-// addresses are uniform and lanes add 32-bit offsets. Smaller ones: lane t holds the page of key t.
+// addresses are uniform and lanes add 32-bit offsets. Smaller ones: lane t holds the page of key t
+// (one token over 777 keys 7.7 and 8.1 us, 2048 over 8192 308 and 312).
 template <bool Large>
 struct StepPages {
     int page[Large ? 2 : 1];
@@ -341,7 +349,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
                                 if (j == slot % 8) va[j] = vt[j], pa[j] = pp[j];
                         }
                         const f32x4 one = T::mfma16(va, pa, f32x4{});
-                        if (sees(now0 + 16 * (slot % 8 / 4) + 4 * (slot / 8) + slot % 4, pos, window, sinks)) o[d] += one;
+                        if (sees(now0 + 16 * (slot % 8 / 4) + 4 * (slot / 8) + slot % 4, pos, window, sinks))
+                            o[d] += one;
                     }
                     continue;
                 }
@@ -358,7 +367,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
     for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int d = 0; d < kLaneDims; d += 4)
-            *(f32x4*)&lds_o[wave][i16][(4 * g + r) * kLaneDims + d] = f32x4{o[d][r], o[d + 1][r], o[d + 2][r], o[d + 3][r]};
+            *(f32x4*)&lds_o[wave][i16][(4 * g + r) * kLaneDims + d] = 
+                f32x4{o[d][r], o[d + 1][r], o[d + 2][r], o[d + 3][r]};
     __syncthreads();
 
     // columns pairwise: thread -> (row, dims 2 c, 2 c + 1)
@@ -369,7 +379,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
     auto put = [&](int r, int c, float x, float y, float top, float sum) {
         const int64_t token = seq.first + r / group, q_head = head * group + r % group;
         const float inv = sum > 0.0f ? 1.0f / sum : sum;   // NaN stays NaN
-        *(uint32_t*)((short*)a.out + token * a.out_token_stride + q_head * a.out_head_stride + c) = T::pack(x * inv, y * inv);
+        *(uint32_t*)((short*)a.out + token * a.out_token_stride + q_head * a.out_head_stride + c) =
+            T::pack(x * inv, y * inv);
         if (a.lse && c == 0) a.lse[token * a.q_heads + q_head] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
     };
     for (int i = threadIdx.x; i < items; i += 64 * kRowWaves) {
@@ -439,18 +450,21 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
 // ---------------------------------------------------------------------------------
 // Many rows
 // ---------------------------------------------------------------------------------
-// One workgroup: 8 (or 4) waves of 32 rows of one sequence and KV head against the keys that they see, 64 at a time through
-// LDS. Products are taken transposed, S^T = K Q^T and O^T = V^T P^T (32 x 32 x 16), so that a lane holds scores of
-// one row only and the P that it computed is already the second product's operand: key slots are permuted alike in P
+// One workgroup: 8 (or 4) waves of 32 rows of one sequence and KV head against the keys that they see, 64 at a time
+// through LDS. Products are taken transposed, S^T = K Q^T and O^T = V^T P^T (32 x 32 x 16), so that a lane holds scores
+// of one row only and the P that it computed is already the second product's operand: key slots are permuted alike in P
 // and V^T, which a sum over keys allows. V^T comes out of LDS by transposing reads.
 //
-// Bound by the matrix cores, LDS reads and exponentials close behind: the scores of the next tile are multiplied
-// while those of this one go through the softmax. Tiles come from memory without passing registers, two buffers
-// each of K and V, one barrier a tile. 4096 tokens over 32768 keys, 32 / 8 heads of 128: 2.1 ms, 980 TFLOP/s
-// (64 rows a wave, 4 waves, one buffer less read: 3.3 ms, its 512 registers leave one wave a SIMD).
+// Bound by the matrix cores and the vector units, which are busy for 45 % of the time each (16 products of 32 cycles
+// and as long a stretch of exponentials, sums and roundings for 32 x 64 scores), at 2.0 to 2.1 GHz under this load: the
+// scores of the next tile are multiplied while those of this one go through the softmax. Tiles come from memory without
+// passing registers, two buffers each of K and V, one barrier a tile. 4096 tokens over 32768 keys, 32 / 8 heads of 128:
+// 2.15 ms in fp16 (960 TFLOP/s; a product of 8192 x 8192 matrices reaches 1180), 2.0 ms in bf16 (1040 of
+// 1240). 64 rows a wave halve the LDS reads, but their 512 registers leave one wave a SIMD: 3.3 ms.
 //
 // Where tiles are few, their keys are split; the parts go to the workspace in fp32 and are joined in order by
-// attention_join_kernel.
+// attention_join_kernel (128 tokens over 32768 keys, 32 / 8 heads of 128: 1019 us whole, 97 in
+// parts).
 template <int D>
 struct Tile {
     // D = 256 needs twice the registers a row; D = 64 has fewer products to a score, and two workgroups of 4 waves on a
@@ -476,7 +490,8 @@ constexpr float kSlack = 8.0f;
 
 struct TilePlan {
     uint32_t splits;       // of a tile, at most
-    uint64_t offset;       // in the workspace: the steps of a split, then from kPartsAt on the parts, [split][token][q head]
+    // in the workspace: the steps of a split, then from kPartsAt on the parts, [split][token][q head]
+    uint64_t offset;
                            // rows of D sums and then their m and l
     uint64_t bytes;
 };
@@ -484,15 +499,17 @@ constexpr uint64_t kPartsAt = 256;
 constexpr uint32_t kLeastChunk = 8;    // steps: a split's part of the sums costs as much as one
 
 // Steps of `unit` keys that rows of up to `span` neighbouring tokens of a sequence see, at most.
-__host__ __device__ inline uint64_t most_steps(uint64_t keys, uint64_t unit, uint64_t span, uint64_t window, uint64_t sinks) {
-    const uint64_t steps = (keys + unit - 1) / unit, some = (window + span + unit - 1) / unit + 1 + (sinks + unit - 1) / unit;
+__host__ __device__ inline uint64_t most_steps(uint64_t keys, uint64_t unit, uint64_t span, uint64_t window,
+                                               uint64_t sinks) {
+    const uint64_t steps = (keys + unit - 1) / unit;
+    const uint64_t some = (window + span + unit - 1) / unit + 1 + (sinks + unit - 1) / unit;
     return window && some < steps ? some : steps;
 }
 
-// The tiles of all sequences and their splits. Only the device knows the lengths, so every wave reads them, 64 sequences
-// at a time. `chunk`, the steps of a split, is the least that makes no more workgroups than run at once: a second round
-// for a few of them costs more than it shortens the first, and so do parts of sums for tiles that fill the card by
-// themselves (4096 tokens over 4096 keys, 16 heads of 64, 256 tiles: 103 us whole, 143 us split into 512).
+// The tiles of all sequences and their splits. Only the device knows the lengths, so every wave reads them, 64
+// sequences at a time. `chunk`, the steps of a split, is the least that makes no more workgroups than run at once: a
+// second round for a few of them costs more than it shortens the first, and so do parts of sums for tiles that fill the
+// card by themselves (4096 tokens over 4096 keys, 16 heads of 64, 256 tiles: 103 us whole, 143 us split into 512).
 template <int D>
 struct TileWork {
     typedef Tile<D> C;
@@ -522,7 +539,8 @@ struct TileWork {
         chunk = max(longest, 1u);
         if (plan.splits == 1 || 2 * tiles > C::kFill) return;
         // no more than 2^8 tiles of fewer than 2^24 steps
-        chunk = max(max((wave_sum(total) * a.kv_heads + C::kFill - 1) / C::kFill, (longest + plan.splits - 1) / plan.splits), kLeastChunk);
+        chunk = max((wave_sum(total) * a.kv_heads + C::kFill - 1) / C::kFill, kLeastChunk);
+        chunk = max(chunk, (longest + plan.splits - 1) / plan.splits);
         for (;;) {   // twice the even share makes at most C::kFill / 2 + tiles
             uint32_t items = 0;
             for (int s0 = 0; s0 < (int)a.sequences; s0 += 64) {
@@ -561,15 +579,16 @@ typedef __attribute__((address_space(3))) char* lds_bytes;
 typedef const __attribute__((address_space(1))) void* global_void;
 
 template <class T, int D, bool Large>
-__global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attention_tile_kernel(const ls_hip_attention a, uint32_t shift,
-                                                                              const TilePlan plan) {
+__global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attention_tile_kernel(
+    const ls_hip_attention a, uint32_t shift, const TilePlan plan) {
     typedef Tile<D> C;
     constexpr int kKeys = C::kKeys, kSub = kKeys / 32;
     __shared__ __align__(1024) short lds_k[2][kKeys * D];
     __shared__ __align__(1024) short lds_v[2][kKeys * D];
 
     TileWork<D> work(a, plan);
-    if (plan.splits > 1 && blockIdx.x == 0 && threadIdx.x == 0) *(uint32_t*)((char*)a.workspace + plan.offset) = work.chunk;
+    if (plan.splits > 1 && blockIdx.x == 0 && threadIdx.x == 0) 
+        *(uint32_t*)((char*)a.workspace + plan.offset) = work.chunk;
     work.find(a, blockIdx.x / a.kv_heads);
     if (work.seq < 0) return;
     const int head = blockIdx.x % a.kv_heads, group = a.q_heads / a.kv_heads;
@@ -658,7 +677,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
     // left of an address is a constant of the instruction.
     const uint32_t k_at = 2 * D * col + 16 * (h ^ C::turn(col));
     const int v_row = 4 * h + (lane & 15) / 4;
-    const uint32_t v_at = 2 * D * v_row + 16 * ((2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ C::turn(v_row)) + 8 * (lane & 1);
+    const uint32_t v_at = 2 * D * v_row + 16 * ((2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ C::turn(v_row)) +
+        8 * (lane & 1);
     auto keys = [&](const lds_bytes lds, int i, s16x8 (&k)[kSub]) LS_INLINE {
         const lds_bytes at = lds + (k_at ^ (32 * i));
 #pragma unroll
@@ -687,7 +707,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
         const lds_bytes lds = (lds_bytes)lds_v + (t & 1) * (2 * D * kKeys);
         typedef __attribute__((address_space(3))) s16x4* lds_ptr;
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (v_at ^ (64 * d)) + 2 * D * 16 * t16));
-        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (v_at ^ (64 * d) ^ 32) + 2 * D * (16 * t16 + 8)));
+        const s16x4 v1 =
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + (v_at ^ (64 * d) ^ 32) + 2 * D * (16 * t16 + 8)));
         return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     auto sees_all = [&](int key0, int low, int high) {   // rows from position low to high see every key of a tile
@@ -701,9 +722,9 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kt][i]);
         return top;
     };
-    // An infinity or NaN in a value must reach only the rows that see its key, and 0 * NaN is NaN: where not every row of
-    // the workgroup sees all keys of a tile, such values become 0. True if one of them belongs to a row that sees it:
-    // it is then added to the result at the end.
+    // An infinity or NaN in a value must reach only the rows that see its key, and 0 * NaN is NaN: where not every row
+    // of the workgroup sees all keys of a tile, such values become 0. True if one of them belongs to a row that sees
+    // it: it is then added to the result at the end.
     auto settle = [&](int t, int key0) {
         bool odd = false, seen = false;
         for (int i = lane; i < kKeys * D / 8; i += 64) odd |= not_finite<T>(*(const s16x8*)(lds_v[t & 1] + 8 * i));
@@ -756,7 +777,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
                 for (int kt = 0; kt < kSub; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (!sees(key0 + 32 * kt + 8 * (i / 4) + 4 * h + i % 4, pos, window, sinks)) s[kt][i] = -INFINITY;
+                        if (!sees(key0 + 32 * kt + 8 * (i / 4) + 4 * h + i % 4, pos, window, sinks))
+                            s[kt][i] = -INFINITY;
                 top = largest(s);
             }
             top = max32(top) * scale;
@@ -767,8 +789,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) o[d] *= keep;
             }
-            // The next tile's scores (after the last one: of what the buffer held before, unused), and this one's P beside
-            // them: rounded to the values' type for the matrix product, summed in fp32.
+            // The next tile's scores (after the last one: of what the buffer held before, unused), and this one's P
+            // beside them: rounded to the values' type for the matrix product, summed in fp32.
             f32x16 next[kSub];
             u32x4 p[kKeys / 16];
             scores(next, t + 1, [&](int step) LS_INLINE {
@@ -792,7 +814,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
 #pragma unroll
                     for (int d = 0; d < D / 32; ++d) v[(t16 + 1) & 1][d] = values(t, t16 + 1, d);
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d) o[d] = T::mfma32(v[t16 & 1][d], __builtin_bit_cast(s16x8, p[t16]), o[d]);
+                for (int d = 0; d < D / 32; ++d)
+                    o[d] = T::mfma32(v[t16 & 1][d], __builtin_bit_cast(s16x8, p[t16]), o[d]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) top = fmaxf(top, next[t16 / 2][t16 % 2 * 8 + i]);
             }
@@ -820,7 +843,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
-                    *(f32x4*)(parts + at * D + 32 * d + 2 * i + 4 * h) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+                    *(f32x4*)(parts + at * D + 32 * d + 2 * i + 4 * h) =
+                        f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
             if (h == 0) *(f32x2*)(parts + part_rows * D + 2 * at) = f32x2{m, l};
         }
     }
@@ -844,7 +868,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
         }
         if (sum == 0.0f) continue;
         if (whole)
-            ((short*)a.out)[(seq.first + its) * a.out_token_stride + its_head * a.out_head_stride + c] = (short)T::pack(sum, 0.0f);
+            ((short*)a.out)[(seq.first + its) * a.out_token_stride + its_head * a.out_head_stride + c] =
+                (short)T::pack(sum, 0.0f);
         else parts[((int64_t)(seq.first + its) * a.q_heads + its_head) * D + c] = sum;
     }
 }
@@ -858,7 +883,8 @@ __global__ __launch_bounds__(1024) void attention_join_kernel(const ls_hip_atten
     // the sequence of token t: the last one that starts at or before it
     int s = 0;
     for (int s0 = 0; s0 < (int)a.sequences; s0 += 64) {
-        const uint64_t before = __ballot(s0 + lane < (int)a.sequences && a.q_start[min(s0 + lane, (int)a.sequences - 1)] <= t);
+        const uint64_t before =
+            __ballot(s0 + lane < (int)a.sequences && a.q_start[min(s0 + lane, (int)a.sequences - 1)] <= t);
         if (!before) break;
         s = s0 + 63 - __clzll((long long)before);
     }
@@ -871,7 +897,8 @@ __global__ __launch_bounds__(1024) void attention_join_kernel(const ls_hip_atten
     if (q_head < (int)a.q_heads) {
         const int row0 = ((t - seq.first) * group + q_head % group) / Tile<D>::kRows * Tile<D>::kRows;
         const int row_end = min(row0 + Tile<D>::kRows, rows);
-        const Steps steps(Tile<D>::kKeys, base + row0 / group, base + (row_end - 1) / group, (int)a.window, (int)a.sinks);
+        const Steps steps(Tile<D>::kKeys, base + row0 / group, base + (row_end - 1) / group, (int)a.window,
+                          (int)a.sinks);
         if (steps.count <= chunk) return;   // one split: the result is written
         const int64_t at = (int64_t)t * a.q_heads + q_head;
         const float* parts = (const float*)((const char*)a.workspace + plan.offset + kPartsAt);
@@ -881,7 +908,8 @@ __global__ __launch_bounds__(1024) void attention_join_kernel(const ls_hip_atten
         for (int begin = 0; begin < steps.count; begin += chunk, parts += part_rows * (D + 2)) {
             const f32x2 ml = *(const f32x2*)(parts + part_rows * D + 2 * at);
             const lane_sums x = *(const lane_sums*)(parts + at * D + kLane * lane);
-            const float next = fmaxf(m, ml[0]), old = __builtin_amdgcn_exp2f(m - next), f = __builtin_amdgcn_exp2f(ml[0] - next);
+            const float next = fmaxf(m, ml[0]), old = __builtin_amdgcn_exp2f(m - next);
+            const float f = __builtin_amdgcn_exp2f(ml[0] - next);
             o = o * old + x * f;
             l = l * old + ml[1] * f;
             m = next;
@@ -898,17 +926,20 @@ bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1
 
 int check(const ls_hip_attention& a) {
     if (!a.q || !a.out || !a.k_pages || !a.v_pages || !a.page_table || !a.q_start || !a.context) return EINVAL;
-    if (!a.sequences || !a.q_heads || !a.kv_heads || a.q_heads % a.kv_heads || !a.pages || !a.table_width) return EINVAL;
+    if (!a.sequences || !a.q_heads || !a.kv_heads || a.q_heads % a.kv_heads || !a.pages || !a.table_width)
+        return EINVAL;
     if (!a.page_size || (a.page_size & (a.page_size - 1)) || a.dtype > LS_TYPE_F32) return EINVAL;
     if (a.tokens > 0x7fffffffu || a.pages > 0x7fffffffu || a.window > 0x3fffffffu || a.sinks > 0x3fffffffu ||
         a.max_context > 0x3fffffffu || (uint64_t)a.table_width * a.page_size < a.max_context || a.max_new > a.tokens)
         return EINVAL;
-    if (a.table_stride < 0 || (a.sequences > 1 && a.table_stride < (int64_t)a.table_width) || !(std::fabs(a.scale) < INFINITY))
+    if (a.table_stride < 0 || (a.sequences > 1 && a.table_stride < (int64_t)a.table_width) ||
+        !(std::fabs(a.scale) < INFINITY))
         return EINVAL;
     if (!aligned(a.q, 16) || !aligned(a.out, 16) || !aligned(a.k_pages, 16) || !aligned(a.v_pages, 16) ||
         !aligned(a.workspace, 16))
         return EINVAL;
-    const int64_t strides[] = {a.q_token_stride, a.q_head_stride, a.out_token_stride, a.out_head_stride, a.k_page_stride,
+    const int64_t strides[] = {a.q_token_stride, a.q_head_stride, a.out_token_stride, a.out_head_stride,
+                               a.k_page_stride,
                                a.k_head_stride, a.k_slot_stride, a.v_page_stride, a.v_head_stride, a.v_slot_stride};
     for (int64_t s : strides)
         if (s < 0 || s % 8) return EINVAL;
@@ -920,14 +951,15 @@ int check(const ls_hip_attention& a) {
     return 0;
 }
 
-// Splits of the sequences that take the row kernel. Long ones make kFill workgroups (131072 keys, 16 groups: 144 us; with
-// half or twice as many 150 and 154). Splits of few steps pay only up to a workgroup a compute unit (32 sequences of 500
-// keys, 256 groups: whole 15 us, in four 20), and one workgroup joins them all: with s steps, about sqrt(2 s) splits
-// cost least (8000 keys: 21 splits 13 us, 63 splits 18). A split has a step for each of its waves.
+// Splits of the sequences that take the row kernel. Long ones make kFill workgroups (131072 keys, 16 groups: 144 us;
+// with half or twice as many 150 and 154). Splits of few steps pay only up to a workgroup a compute unit (32 sequences
+// of 500 keys, 256 groups: whole 15 us, in four 20), and one workgroup joins them all: with s steps, about sqrt(2 s)
+// splits cost least (8000 keys: 21 splits 13 us, 63 splits 18). A split has a step for each of its waves.
 SplitPlan plan_rows(const ls_hip_attention& a) {
     SplitPlan p{};
     p.rows = (uint32_t)std::min<uint64_t>((uint64_t)a.max_new * (a.q_heads / a.kv_heads), kRows);
-    const uint64_t steps = most_steps(a.max_context, kStepKeys, kRows, a.window, a.sinks), groups = (uint64_t)a.sequences * a.kv_heads;
+    const uint64_t steps = most_steps(a.max_context, kStepKeys, kRows, a.window, a.sinks);
+    const uint64_t groups = (uint64_t)a.sequences * a.kv_heads;
     const auto even = [&](uint64_t workgroups) { return (steps * groups + workgroups - 1) / workgroups; };
     uint64_t chunk = std::max(even(kFill), (steps + kMaxSplits - 1) / kMaxSplits);
     chunk = std::max(chunk, std::min<uint64_t>(even(kFill / 4), 16));
@@ -944,11 +976,13 @@ TilePlan plan_tiles(const ls_hip_attention& a, uint64_t offset) {
     typedef Tile<D> C;
     TilePlan p{};
     const uint64_t group = a.q_heads / a.kv_heads;
-    const uint64_t least = std::max<uint64_t>(1, a.tokens * group / C::kRows) * a.kv_heads;   // workgroups without splits
+    // workgroups without splits
+    const uint64_t least = std::max<uint64_t>(1, a.tokens * group / C::kRows) * a.kv_heads;
     const uint64_t steps = most_steps(a.max_context, C::kKeys, C::kRows / group + 2, a.window, a.sinks);
     p.splits = (uint32_t)std::max<uint64_t>(1, std::min(C::kFill / least, (steps + kLeastChunk - 1) / kLeastChunk));
     p.offset = (offset + 255) / 256 * 256;
-    if (p.splits > 1) p.bytes = p.offset + kPartsAt + p.splits * (uint64_t)a.tokens * a.q_heads * (a.head_dim + 2) * sizeof(float);
+    const uint64_t part = (uint64_t)a.tokens * a.q_heads * (a.head_dim + 2) * sizeof(float);
+    if (p.splits > 1) p.bytes = p.offset + kPartsAt + p.splits * part;
     return p;
 }
 // Workgroups of the tiles: every tile ends with a split that is not full.
@@ -984,13 +1018,15 @@ void launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
     const uint32_t shift = __builtin_ctz(a.page_size);
     if (plan.by_rows) {
         const dim3 grid(plan.rows.splits * a.kv_heads, a.sequences);
-        if (a.page_size >= 16) attention_rows_kernel<T, D, true><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan.rows);
+        if (a.page_size >= 16)
+            attention_rows_kernel<T, D, true><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan.rows);
         else attention_rows_kernel<T, D, false><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan.rows);
     }
     if (plan.by_tiles) {
         typedef Tile<D> C;
         const uint32_t grid = tile_grid<D>(a);
-        if (a.page_size >= 16) attention_tile_kernel<T, D, true><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
+        if (a.page_size >= 16)
+            attention_tile_kernel<T, D, true><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
         else attention_tile_kernel<T, D, false><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
         if (plan.tiles.splits > 1)
             attention_join_kernel<T, D><<<dim3(a.tokens, (a.q_heads + 15) / 16), 1024, 0, stream>>>(a, plan.tiles);

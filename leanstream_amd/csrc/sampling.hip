@@ -4,18 +4,23 @@
 // kept tokens are a prefix of the ranking: everything above a cut logit, and of the tokens equal to it the
 // first few by id. Weights of a set are summed as whole numbers, so no order of atomics changes a result.
 //
-// One pass over the logits, in two launches. A workgroup of the first takes a chunk of a row and leaves its best token, the sum of its
-// exponentials and, in order of id, its candidates: as many of its largest logits as the record holds. A workgroup of
-// the second takes a row: it finds the cuts of top-k and of top-p among the candidates by radix
-// selection (parts of the range of their 32-bit order, with the count and the weight of each).
-// Whatever lies above the largest logit that is no candidate (`outside`) is known completely. Where a cut falls
-// below:
+// One pass over the logits, in two launches. A workgroup of the first takes a chunk of a row and leaves its best token,
+// the sum of its exponentials and, in order of id, its candidates: as many of its largest logits as the record holds.
+// A workgroup of the second takes a row: it finds the cuts of top-k and of top-p among the candidates by radix
+// selection (parts of the range of their 32-bit order, with the count and the weight of each). Whatever lies above the
+// largest logit that is no candidate (`outside`) is known completely. Where a cut falls below:
 //  - top-p alone: the chunks also left histograms of count and weight over bins of T / 16. They name the bin of
 //    the cut, whose tokens are picked from the row (one pass of comparisons) and selected among; the chunks'
 //    weights above the cut point to the chunk that holds the token, and only that is read again;
 //  - otherwise (top-k beyond the candidates, a bin of more tokens than there is room for) the workgroup selects
 //    over the whole row.
 // Without filters the chunks' sums point to the chunk that holds the token.
+//
+// Bound by the waits between the steps of a workgroup: 256 rows of 50257 fp32 logits with top-k take 20 + 11 us for
+// 51 MB (a greedy pick, which needs none of the steps, 13), one row of 32768 7 + 9. A row whose nucleus is wide costs
+// most: 64 rows of 131072, each with settings of its own, 13 + 37 us. One launch, in which a row's last chunk went on
+// with the row, gave the chunks half the waves (its registers): 73 us for 64 rows with top-k, where the first form in
+// two took 28 (now 22).
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cerrno>
@@ -146,8 +151,9 @@ __device__ __forceinline__ V block_before(V x, V* scratch, V* total) {
 
 // The shortest prefix within `limit` whose count reaches need_count or whose weight reaches need_weight, of the
 // tokens with an order in [base, high] that each(f) hands to f(order, weight); all of `limit` if none does.
-// kept: the weight of that prefix. Few: of at most 2^13 tokens, whose count and weight go into one word. A limit with fewer ties than there are must weigh need_weight. Every pass counts the 256 equal parts of the range and goes on with the one
-// in which a sum is reached, until it is one logit or holds so few tokens that one wave ranks them.
+// kept: the weight of that prefix. Few: of at most 2^13 tokens, whose count and weight go into one word. A limit with
+// fewer ties than there are must weigh need_weight. Every pass counts the 256 equal parts of the range and goes on with
+// the one in which a sum is reached, until it is one logit or holds so few tokens that one wave ranks them.
 template <bool Few, class Each>
 __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t high, Cut limit, uint32_t need_count,
                                       uint64_t need_weight, Shared& sh, uint64_t* kept) {
@@ -178,7 +184,8 @@ __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t 
                 w[i] = sh.weights[d];
                 n[i] = Few ? (uint32_t)(w[i] >> kCountShift) : sh.counts[d];
                 if (Few) w[i] &= kWeight;
-                if (shift == 0 && base + d == limit.order && n[i] > limit.ties) w[i] = w[i] / n[i] * limit.ties, n[i] = limit.ties;
+                if (shift == 0 && base + d == limit.order && n[i] > limit.ties)
+                    w[i] = w[i] / n[i] * limit.ties, n[i] = limit.ties;
                 c += n[i];
                 s += w[i];
             }
@@ -191,7 +198,8 @@ __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (digit != 256) continue;
-                    if (reached && n[i] && (c_before + n[i] >= need_count || s_before + w[i] >= need_weight)) digit = 255 - 4 * lane - i;
+                    if (reached && n[i] && (c_before + n[i] >= need_count || s_before + w[i] >= need_weight))
+                        digit = 255 - 4 * lane - i;
                     else c_before += n[i], s_before += w[i];
                 }
                 sh.digit = digit;
@@ -241,7 +249,8 @@ __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t 
                                  (c + equal >= need_count || s + (uint64_t)equal * weight >= need_weight);
             const uint64_t at = __ballot(reached);
             if (threadIdx.x == (uint32_t)__ffsll((unsigned long long)at) - 1) {
-                const uint64_t ties = min(min((uint64_t)equal, (uint64_t)(need_count - c)), (need_weight - s - 1) / weight + 1);
+                const uint64_t ties = min(min((uint64_t)equal, (uint64_t)(need_count - c)),
+                                          (need_weight - s - 1) / weight + 1);
                 sh.before_count = order;
                 sh.before_weight = s + ties * weight;
                 sh.turn = (uint32_t)ties;
@@ -270,8 +279,9 @@ struct RowArgs {
 // The token of the row whose kept tokens, in order of id, are those above the cut and its first ties, with
 // e >= min_p: over all of the row's logits.
 template <class T>
-__device__ __forceinline__ void draw_from_row(const T* logits, uint32_t vocab, float top, const Scale& scale, Cut cut, float min_p,
-                              float uniform, Shared& sh, uint32_t* token, uint64_t* total) {
+__device__ __forceinline__ void draw_from_row(const T* logits, uint32_t vocab, float top, const Scale& scale, Cut cut,
+                                              float min_p, float uniform, Shared& sh, uint32_t* token,
+                                              uint64_t* total) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t stretch = ((vocab + kWaves - 1) / kWaves + 63) / 64 * 64;
     const uint32_t begin = min(wave * stretch, vocab), end = min(begin + stretch, vocab);
@@ -332,8 +342,9 @@ __device__ __forceinline__ void draw_from_row(const T* logits, uint32_t vocab, f
 // The token of a chunk at which the running weight of its kept tokens (units of the row's best one) passes
 // `rest`; ties_before: tokens equal to the cut in earlier chunks.
 template <class T, uint32_t Chunk>
-__device__ __forceinline__ uint32_t draw_from_chunk(const T* logits, uint32_t vocab, uint32_t chunk, float top, const Scale& scale, Cut cut,
-                                    uint32_t ties_before, double rest, Shared& sh) {
+__device__ __forceinline__ uint32_t draw_from_chunk(const T* logits, uint32_t vocab, uint32_t chunk, float top,
+                                                    const Scale& scale, Cut cut, uint32_t ties_before, double rest,
+                                                    Shared& sh) {
     constexpr uint32_t kEach = Chunk / kThreads;
     const uint32_t from = chunk * Chunk + threadIdx.x * kEach;
     float x[kEach];
@@ -485,7 +496,8 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
                 mine += e;
                 const int down = top_bin - scale.bin(x);
                 if (binned && down < kBins)
-                    atomicAdd((unsigned long long*)&sh.bins[down], 1ull << kCountShift | scale.weight_of(e, x == chunk_top));
+                    atomicAdd((unsigned long long*)&sh.bins[down], 
+                              1ull << kCountShift | scale.weight_of(e, x == chunk_top));
             }
         sum = wave_sum((double)mine * 0x1p-32);
         if (lane == 0) sh.wave_sum[wave] = sum;
@@ -499,7 +511,8 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
         while (hits) {
             const uint32_t at = __ffs(hits) - 1;
             hits &= hits - 1;
-            const int down = top_bin - scale.bin(to_float(logits[begin + 8 * (at / 8 * kThreads + threadIdx.x) + at % 8]));
+            const uint32_t from = begin + 8 * (at / 8 * kThreads + threadIdx.x) + at % 8;
+            const int down = top_bin - scale.bin(to_float(logits[from]));
             if (down < kBins) atomicAdd((unsigned long long*)&sh.bins[down], 1ull << kCountShift);
         }
     }
@@ -522,9 +535,12 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
             for (int i = 0; i < kBins / 64; ++i) n += (uint32_t)(sh.bins[kBins / 64 * lane + i] >> kCountShift);
             uint32_t upto = wave_upto(n) - n;
 #pragma unroll
-            for (int i = 0; i < kBins / 64; ++i) fit += (upto += (uint32_t)(sh.bins[kBins / 64 * lane + i] >> kCountShift)) <= rows.room;
+            for (int i = 0; i < kBins / 64; ++i)
+                fit += (upto += (uint32_t)(sh.bins[kBins / 64 * lane + i] >> kCountShift)) <= rows.room;
             fit = wave_sum(fit);
-            if (lane == 0) sh.digit = summed || mean == -INFINITY ? fit : min(fit, (uint32_t)max(0, min(top_bin - scale.bin(mean), kBins)));
+            if (lane == 0)
+                sh.digit = summed || mean == -INFINITY
+                               ? fit : min(fit, (uint32_t)max(0, min(top_bin - scale.bin(mean), kBins)));
         }
         __syncthreads();
         const int bins = (int)sh.digit;
@@ -599,7 +615,11 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
     float outside = __uint_as_float((uint32_t)tail);
     outside = wave_max(outside, -INFINITY);
     if (lane == 0) sh.wave_float[wave] = outside;
-    if (mine) sh.tops[threadIdx.x] = logit_of((uint32_t)(own >> 32)), sh.sums[threadIdx.x] = sum, sh.held[threadIdx.x] = (uint32_t)(tail >> 32);
+    if (mine) {
+        sh.tops[threadIdx.x] = logit_of((uint32_t)(own >> 32));
+        sh.sums[threadIdx.x] = sum;
+        sh.held[threadIdx.x] = (uint32_t)(tail >> 32);
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) outside = fmaxf(outside, sh.wave_float[i]);
@@ -724,11 +744,13 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
             __syncthreads();
             if (sh.before_count > kCandidates) return false;
             const uint64_t need = sh.before_weight;
-            // The ids of its tokens, in any order, into the slots of the candidates (which are all read). A thread marks
-            // what it finds among 64 logits before it takes slots: one by one, the few hits of every wave would each
-            // wait for the counter.
+            // The ids of its tokens, in any order, into the slots of the candidates (which are all read). A thread
+            // marks what it finds among 64 logits before it takes slots: one by one, the few hits of every wave would
+            // each wait for the counter.
             const float least = scale.first_of(row_bin - (int)bin), beyond = scale.first_of(row_bin - (int)bin + 1);
-            auto slot_at = [&](uint32_t slot) LS_INLINE { return record + slot / rows.room * words + kHead + slot % rows.room; };
+            auto slot_at = [&](uint32_t slot) LS_INLINE {
+                return record + slot / rows.room * words + kHead + slot % rows.room;
+            };
             constexpr uint32_t kDeep = 8;
             const uint32_t room = rows.room * rows.chunks, whole = a.vocab / 8;
             for (uint32_t i0 = threadIdx.x; i0 <= whole; i0 += kDeep * kThreads) {
@@ -792,7 +814,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
             __syncthreads();
 #pragma unroll
             for (uint32_t i = 0; i < kSlots; ++i) {
-                if (weight[i] && order[i] > cut.order) atomicAdd((unsigned long long*)&sh.list[id[i] / kChunk], (unsigned long long)weight[i]);
+                if (weight[i] && order[i] > cut.order)
+                    atomicAdd((unsigned long long*)&sh.list[id[i] / kChunk], (unsigned long long)weight[i]);
                 if (weight[i] && order[i] == cut.order) atomicAdd(&sh.held[id[i] / kChunk], 1u);
             }
             for (uint32_t c = wave; c < rows.chunks; c += kWaves) {
@@ -815,8 +838,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
             double part = 0.0;
             if (mine) {
                 const uint32_t admitted = min(ties, cut.ties - min(cut.ties, ties_before));
-                part = sh.sums[threadIdx.x] +
-                       (double)(sh.list[threadIdx.x] + (uint64_t)admitted * scale.weight(logit_of(cut.order), top)) * 0x1p-32;
+                const uint64_t tied = (uint64_t)admitted * scale.weight(logit_of(cut.order), top);
+                part = sh.sums[threadIdx.x] + (double)(sh.list[threadIdx.x] + tied) * 0x1p-32;
             }
             token = pick(part, cut, ties_before, &bin_kept);
             return true;
@@ -854,7 +877,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
             kept = bin_kept;
         } else {
             cut = all;
-            if (by_count || by_weight) cut = select<false>(everything, low, high, cut, by_count ? set.top_k : kAll, ~0ull, sh, &total);
+            if (by_count || by_weight)
+                cut = select<false>(everything, low, high, cut, by_count ? set.top_k : kAll, ~0ull, sh, &total);
             if (by_weight) {
                 const uint64_t limit = share(total, top_p, true);
                 cut = select<false>(everything, low, high, cut, kAll, limit ? limit : 1, sh, &total);
@@ -876,7 +900,8 @@ bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1
 int check(const ls_hip_sample& a) {
     if (!a.logits || !a.uniform || !a.tokens || !a.vocab || a.dtype > LS_TYPE_F32) return EINVAL;
     if (!aligned(a.logits, a.dtype == LS_TYPE_F32 ? 4 : 2) || a.row_stride < 0) return EINVAL;
-    for (const void* p : {(const void*)a.uniform, (const void*)a.temperature, (const void*)a.top_k, (const void*)a.top_p,
+    for (const void* p : {(const void*)a.uniform, (const void*)a.temperature, (const void*)a.top_k,
+         (const void*)a.top_p,
                           (const void*)a.min_p, (const void*)a.tokens, (const void*)a.logprob})
         if (!aligned(p, 4)) return EINVAL;
     if (!aligned(a.workspace, 16)) return EINVAL;
@@ -884,8 +909,9 @@ int check(const ls_hip_sample& a) {
     return 0;
 }
 
-// Chunks of 4096 logits while the rows are few (less than one workgroup a compute unit with twice as many),
-// of 8192 otherwise; a row's candidates are shared out evenly.
+// Chunks of 4096 logits while the rows are few (less than one workgroup a compute unit with twice as many), of 8192
+// otherwise: top-p of one row of 32768 15.4 us with 4096 and 16.3 with 8192, of 131072 16.7 and 17.7; of 64 rows of
+// 131072 30.0 and 26.6. A row's candidates are shared out evenly.
 RowArgs plan_rows(const ls_hip_sample& a, int* vecs) {
     RowArgs p{};
     const uint32_t twice = (a.vocab + 16 * kThreads - 1) / (16 * kThreads);
