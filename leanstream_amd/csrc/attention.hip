@@ -980,7 +980,7 @@ TilePlan plan_tiles(const ls_hip_attention& a, uint64_t offset) {
     const uint64_t least = std::max<uint64_t>(1, a.tokens * group / C::kRows) * a.kv_heads;
     const uint64_t steps = most_steps(a.max_context, C::kKeys, C::kRows / group + 2, a.window, a.sinks);
     p.splits = (uint32_t)std::max<uint64_t>(1, std::min(C::kFill / least, (steps + kLeastChunk - 1) / kLeastChunk));
-    p.offset = (offset + 255) / 256 * 256;
+    p.offset = (std::max(offset, kCounterBytes) + 255) / 256 * 256;   // a call of few rows may use the counters next
     const uint64_t part = (uint64_t)a.tokens * a.q_heads * (a.head_dim + 2) * sizeof(float);
     if (p.splits > 1) p.bytes = p.offset + kPartsAt + p.splits * part;
     return p;

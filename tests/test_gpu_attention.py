@@ -326,6 +326,21 @@ def test_one_workspace_for_calls_of_every_shape(torch_gpu):
         p.check()
 
 
+def test_a_workspace_after_calls_without_row_splits(torch_gpu):
+    """A call that only splits tiles leaves the counters of later calls' splits alone."""
+    torch = torch_gpu
+    chunk = Problem(torch, "bfloat16", 64, 40, 1, 16, [(30, 2000), (17, 900)])    # no sequence of few rows
+    one = Problem(torch, "bfloat16", 128, 8, 2, 16, [(1, 6000)])
+    need = max(p.on_gpu().workspace.numel() for p in (chunk, one))
+    shared = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    calls = [p.on_gpu(workspace=shared) for p in (chunk, one)]
+    for _ in range(2):
+        for c in calls:
+            c.enqueue()
+    for p in (chunk, one):
+        p.check()
+
+
 def test_long_split_sequences(torch_gpu):
     """Many splits of few rows and of tiles: one long sequence alone, and long ones among short ones."""
     torch = torch_gpu
