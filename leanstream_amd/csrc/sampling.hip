@@ -73,7 +73,7 @@ struct Scale {
         const double c = 1.4426950408889634 / (double)temperature;
         hi = (float)c;
         lo = hi < INFINITY ? (float)(c - (double)hi) : 0.0f;
-        bins = fminf(16.0f / temperature, 3e38f);
+        bins = fmaxf(fminf(16.0f / temperature, 3e38f), 0x1p-126f);   // never 0: inf * 0 has no place among the bins
     }
     // bin on the scale of all logits of a row, rising with the logit
     __device__ __forceinline__ float steps(float l) const { return fminf(fmaxf(floorf(l * bins), -1e9f), 1e9f); }
@@ -226,7 +226,7 @@ __device__ __forceinline__ Cut select(const Each& each, uint32_t base, uint32_t 
             return Cut{base + digit, (uint32_t)ties};
         }
         base += digit << shift;
-        high = min(high, base + ((1u << shift) - 1));
+        high = base + min(high - base, (1u << shift) - 1);
         if (n > 64) continue;
         each([&](uint32_t order, uint32_t weight) LS_INLINE {
             if (!weight || order < base || order > high) return;
@@ -568,6 +568,9 @@ __global__ __launch_bounds__(kThreads) void sample_chunk_kernel(const ls_hip_sam
         // candidates in order of id: a thread takes 32 elements' marks
         uint32_t word = threadIdx.x < kChunk / 32 ? ((const uint32_t*)marks)[threadIdx.x] : 0u, total;
         uint32_t at = block_before((uint32_t)__popc(word), sh.wave32, &total);
+        // Bins beyond 2^24 (a tiny temperature) are not exact and infinite logits share the last: a chunk whose
+        // candidates would not fit leaves none.
+        if (total > rows.room) word = 0, total = 0, outside = chunk_top;
         while (word) {
             const uint32_t id = begin + 32 * threadIdx.x + __ffs(word) - 1;
             word &= word - 1;
@@ -901,8 +904,7 @@ int check(const ls_hip_sample& a) {
     if (!a.logits || !a.uniform || !a.tokens || !a.vocab || a.dtype > LS_TYPE_F32) return EINVAL;
     if (!aligned(a.logits, a.dtype == LS_TYPE_F32 ? 4 : 2) || a.row_stride < 0) return EINVAL;
     for (const void* p : {(const void*)a.uniform, (const void*)a.temperature, (const void*)a.top_k,
-         (const void*)a.top_p,
-                          (const void*)a.min_p, (const void*)a.tokens, (const void*)a.logprob})
+                          (const void*)a.top_p, (const void*)a.min_p, (const void*)a.tokens, (const void*)a.logprob})
         if (!aligned(p, 4)) return EINVAL;
     if (!aligned(a.workspace, 16)) return EINVAL;
     if (a.vocab > kMaxVocab || a.rows > 0x7fffffffu) return ENOTSUP;

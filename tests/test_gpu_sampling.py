@@ -196,6 +196,33 @@ def test_extreme_settings(torch_gpu):
     check(torch, logits, u, [math.inf] * 8)
 
 
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_many_infinite_logits(torch_gpu, dtype):
+    """More infinite logits than a chunk has room for, at any temperature: they share the row."""
+    torch = torch_gpu
+    logits, u, g = random_rows(torch, 4, 20000, dtype, 8)
+    for r, n in enumerate((300, 6000, 20000, 1)):
+        logits[r, torch.randperm(20000, generator=g)[:n]] = math.inf
+    for t in (None, [math.inf] * 4, [1e-6] * 4):
+        for k, p, m in (([10] * 4, None, None), (None, [0.5] * 4, None), ([400] * 4, [0.9] * 4, None), (None, None, [0.5] * 4)):
+            check(torch, logits, u, t, k, p, m)
+
+
+def test_neighbouring_logits_at_tiny_temperatures(torch_gpu):
+    """Logits a unit in the last place apart, of weights that still compare, many of each."""
+    torch = torch_gpu
+    near = 10.0 - 2.0 ** -20
+    g = torch.Generator().manual_seed(12)
+    logits = torch.randn(4, 20000, generator=g)
+    for r, (few, many) in enumerate(((10, 6000), (1, 8000), (100, 250), (3, 15000))):
+        at = torch.randperm(20000, generator=g)
+        logits[r, at[:few]] = 10.0
+        logits[r, at[few:few + many]] = near
+    u = torch.rand(4, generator=g).tolist()
+    for k, p, m in (([20] * 4, None, None), (None, [0.5] * 4, None), ([400] * 4, [0.9] * 4, None), (None, None, [0.3] * 4)):
+        check(torch, logits.cuda(), u, [1e-6] * 4, k, p, m)
+
+
 def test_rows_of_any_stride_and_alignment(torch_gpu):
     torch = torch_gpu
     for dtype in (torch.float16, torch.float32):
