@@ -286,9 +286,10 @@ enum { LS_TYPE_F16 = 0, LS_TYPE_BF16 = 1, LS_TYPE_F32 = 2 };
  * Query head h reads KV head h / (q_heads / kv_heads). Key j of sequence s is slot j % page_size of page
  * page_table[s * table_stride + j / page_size]; entries of pages that no token sees are not read as pages
  * (any value). Slots that a token does not see do not change its result, whatever they hold. A sequence
- * whose lengths are out of bounds counts as one with no keys (status RANGE); a key in a page outside
- * [0, pages) as a key and value of zeros (status BAD_DESCRIPTOR).
- * head_dim 64, 128 or 256; page_size a power of two; F16 or BF16 throughout; every pointer 16-byte
+ * whose context is out of bounds counts as one with no keys, one whose q_start is out of bounds as one with
+ * no tokens, whose rows of out stay as they are (both: status RANGE); a key in a page outside [0, pages)
+ * counts as a key and value of zeros (status BAD_DESCRIPTOR).
+ * scale > 0; head_dim 64, 128 or 256; page_size a power of two; F16 or BF16 throughout; every pointer 16-byte
  * aligned and strides multiples of 8. The workspace (ls_hip_attention_workspace bytes, zeroed once by the
  * caller, then left alone) may be shared by calls that follow one another on one stream. */
 typedef struct ls_hip_attention {
@@ -374,7 +375,8 @@ int ls_hip_block_norm_enqueue(const ls_hip_block_norm* norm, void* stream);
  * -inf; a row without a logit above -inf gives token -1 and logprob -inf. logprob (optional): the logarithm of
  * e_token over the kept weight.
  * temperature, top_k, top_p, min_p: per row, or NULL for 1, all, 1, 0. vocab <= 2^20.
- * The workspace: as for attention, of ls_hip_sample_workspace bytes. */
+ * The workspace (ls_hip_sample_workspace bytes, any contents) may be shared by calls of this kind that follow
+ * one another on one stream, not with attention's. */
 typedef struct ls_hip_sample {
     const void* logits;           /* [rows][vocab], F16, BF16 or F32 */
     const float* uniform;         /* [rows] in [0, 1) */

@@ -933,8 +933,11 @@ int check(const ls_hip_attention& a) {
         a.max_context > 0x3fffffffu || (uint64_t)a.table_width * a.page_size < a.max_context || a.max_new > a.tokens)
         return EINVAL;
     if (a.table_stride < 0 || (a.sequences > 1 && a.table_stride < (int64_t)a.table_width) ||
-        !(std::fabs(a.scale) < INFINITY))
+        !(a.scale > 0.0f && a.scale < INFINITY))
         return EINVAL;
+    for (const void* p : {(const void*)a.page_table, (const void*)a.q_start, (const void*)a.context, (const void*)a.lse,
+                          (const void*)a.status})
+        if (!aligned(p, 4)) return EINVAL;
     if (!aligned(a.q, 16) || !aligned(a.out, 16) || !aligned(a.k_pages, 16) || !aligned(a.v_pages, 16) ||
         !aligned(a.workspace, 16))
         return EINVAL;

@@ -298,6 +298,9 @@ int check(const ls_hip_append& a) {
     if (a.table_stride < 0 || (a.sequences > 1 && a.table_stride < (int64_t)a.table_width)) return EINVAL;
     for (const void* p : {a.q, a.k, a.v, (const void*)a.q_out, (const void*)a.k_pages, (const void*)a.v_pages})
         if (!aligned(p, 2)) return EINVAL;
+    for (const void* p : {(const void*)a.cos, (const void*)a.sin, (const void*)a.page_table, (const void*)a.q_start,
+                          (const void*)a.context, (const void*)a.status})
+        if (!aligned(p, 4)) return EINVAL;
     const int64_t strides[] = {a.q_token_stride, a.q_head_stride, a.k_token_stride, a.k_head_stride, a.v_token_stride,
                                a.v_head_stride, a.q_out_token_stride, a.q_out_head_stride, a.k_page_stride,
                                a.k_head_page_stride, a.k_slot_stride, a.v_page_stride, a.v_head_page_stride,

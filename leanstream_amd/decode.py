@@ -104,7 +104,7 @@ def _check_sequences(page_table, q_start, context, status):
 
 class PagedAttention(_Call):
     """out [tokens, q_heads, head_dim]: attention of the new tokens q over their sequences' keys in `cache`.
-    max_new and max_context bound a sequence's new tokens and keys; scale defaults to head_dim ** -0.5;
+    max_new and max_context bound a sequence's new tokens and keys; scale (> 0) defaults to head_dim ** -0.5;
     window and sinks restrict a token to its last `window` keys and the sequence's first `sinks`. lse
     (optional, fp32 [tokens, q_heads]) gets the logarithm of every row's softmax sum."""
 

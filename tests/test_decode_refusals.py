@@ -105,3 +105,18 @@ def test_classes_refuse_tensors_off_the_gpu():
         decode.BlockNorm(pages[0, 0], pages[0, 0], pages[0, 0], None)
     with pytest.raises(ValueError, match="not on the GPU"):
         decode.Sampler(torch.zeros(1, 8), torch.zeros(1), torch.zeros(1, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("name,make,fields", [
+    ("attention", attention, ["page_table", "q_start", "context", "lse", "status"]),
+    ("append", append, ["cos", "sin", "page_table", "q_start", "context", "status"])])
+def test_words_off_their_alignment_are_refused(name, make, fields):
+    call = getattr(_native.library(), f"ls_hip_{name}_enqueue")
+    for field in fields:
+        assert call(C.byref(make(**{field: 0x9002})), None) == EINVAL, field
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+def test_scales_that_are_not_positive_are_refused(scale):
+    """Masks and maxima are taken before the scale."""
+    assert _native.library().ls_hip_attention_enqueue(C.byref(attention(scale=scale)), None) == EINVAL
