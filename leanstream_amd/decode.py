@@ -57,6 +57,11 @@ class _Call:
         self._device = next(t for t in keep if t is not None).device
         import torch
 
+        if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()):
+            raise ValueError("workspace is a contiguous tensor of bytes")
+        if any(t.device != self._device for t in (*keep, workspace) if t is not None):
+            raise ValueError(f"tensors on more than one device, or off the GPU: {self._device} expected")
+
         # the handle alone: torch.cuda.current_stream() makes an object of it first, 1.9 us of a 3.5 us call
         self._current = functools.partial(torch._C._cuda_getCurrentRawStream, self._device.index)
         need = int(getattr(lib, f"ls_hip_{name}_workspace")(self._arg)) if hasattr(block, "workspace") else 0
@@ -119,8 +124,8 @@ class PagedAttention(_Call):
         if lse is not None and not lse.is_contiguous():
             raise ValueError("lse is not contiguous")
         _check_sequences(page_table, q_start, context, status)
-        if window < 0 or sinks < 0:
-            raise ValueError("window and sinks are 0 or more")
+        if not all(0 <= x < 1 << 30 for x in (window, sinks, max_new, max_context)):
+            raise ValueError("window, sinks, max_new and max_context lie in [0, 2^30)")
         block = _native.Attention(
             q=_ptr(q), out=_ptr(out), lse=_ptr(lse), k_pages=_ptr(cache.k), v_pages=_ptr(cache.v),
             page_table=_ptr(page_table), q_start=_ptr(q_start), context=_ptr(context), status=_ptr(status),

@@ -311,6 +311,20 @@ def test_wrong_tensors_are_refused(torch_gpu):
         p.on_gpu()
 
 
+def test_workspaces_and_bounds_that_do_not_fit_are_refused(torch_gpu):
+    """Decided when the call is bound: a workspace off the GPU or of other elements, numbers beyond 32 bits."""
+    torch = torch_gpu
+    p = Problem(torch, "float16", **CASES["few_tokens"])
+    with pytest.raises(ValueError, match="off the GPU"):
+        p.on_gpu(workspace=torch.zeros(1 << 20, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="bytes"):
+        p.on_gpu(workspace=torch.zeros(1 << 20, device="cuda"))
+    for name in ("window", "sinks", "max_new", "max_context"):
+        for value in (-1, 1 << 30, (1 << 32) + 8):
+            with pytest.raises(ValueError, match="lie in"):
+                p.on_gpu(**{name: value})
+
+
 def test_one_workspace_for_calls_of_every_shape(torch_gpu):
     """Calls that follow one another on a stream share a workspace, whatever each leaves in it."""
     torch = torch_gpu
