@@ -484,8 +484,8 @@ struct Tile {
         return D == 64 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3);
     }
 };
-// The running maximum moves only where a score exceeds it by more than this (base 2): until then P is at most
-// 2^8 instead of 1, and the sums need no scaling.
+// A row's running maximum moves only where one of its scores (times scale log2(e)) exceeds it by more than this: until
+// then P is at most 2^8 instead of 1, and the sums need no scaling.
 constexpr float kSlack = 8.0f;
 
 struct TilePlan {
@@ -783,7 +783,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
             }
             top = max32(top) * scale;
             if (__any(top > m + kSlack)) {
-                const float next_m = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - next_m);
+                // by a row's own scores: with the others' its roundings would hang on keys that it does not see
+                const float next_m = top > m + kSlack ? top : m, keep = __builtin_amdgcn_exp2f(m - next_m);
                 m = next_m;
                 l *= keep;
 #pragma unroll
