@@ -340,13 +340,19 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
                 for (int j = 0; j < 8; ++j) vt[j] = v[j][d];
                 o[d] *= keep;
                 if (!full && __ballot(not_finite<T>(vt))) {
-                    // as in attention_tile_kernel: key by key, each added where it is seen
+                    // A value that is not finite counts as 0 in the product (0 * NaN is NaN); key by key it is then added
+                    // where it is seen. What another row sees does not change the order of a row's sums.
+                    s16x8 odd = {};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (((uint32_t)vt[j] & T::kExponent) == T::kExponent) odd[j] = vt[j], vt[j] = 0;
+                    o[d] = T::mfma16(vt, pp, o[d]);
                     for (int slot = 0; slot < 32; ++slot) {
                         s16x8 va = {}, pa = {};
                         if (g == slot / 8) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
-                                if (j == slot % 8) va[j] = vt[j], pa[j] = pp[j];
+                                if (j == slot % 8) va[j] = odd[j], pa[j] = pp[j];
                         }
                         const f32x4 one = T::mfma16(va, pa, f32x4{});
                         if (sees(now0 + 16 * (slot % 8 / 4) + 4 * (slot / 8) + slot % 4, pos, window, sinks))

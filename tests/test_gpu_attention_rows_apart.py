@@ -62,3 +62,10 @@ def unseen_slots(torch_gpu, shape, dtype, kind):
 @pytest.mark.parametrize("shape", TILES)
 def test_tiles_of_rows(torch_gpu, shape, dtype, kind):
     unseen_slots(torch_gpu, shape, dtype, kind)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("kind", ["large", math.inf, math.nan])
+@pytest.mark.parametrize("shape", ROWS)
+def test_few_rows(torch_gpu, shape, dtype, kind):
+    unseen_slots(torch_gpu, shape, dtype, kind)
