@@ -855,7 +855,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
             if (h == 0) *(f32x2*)(parts + part_rows * D + 2 * at) = f32x2{m, l};
         }
     }
-    // The values that became 0: their sum takes the place of the result of every row that sees one.
+    // The values that became 0: their sum takes the place of the result of every row that sees one, or is added to it
+    // where values of other tiles already left it without a finite one.
     if (!later) return;
     __syncthreads();   // the results are stored
     for (int i = threadIdx.x; i < (row_end - row0) * D; i += 64 * C::kWaves) {
@@ -874,10 +875,12 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
             }
         }
         if (sum == 0.0f) continue;
-        if (whole)
-            ((short*)a.out)[(seq.first + its) * a.out_token_stride + its_head * a.out_head_stride + c] =
-                (short)T::pack(sum, 0.0f);
-        else parts[((int64_t)(seq.first + its) * a.q_heads + its_head) * D + c] = sum;
+        short* out = (short*)a.out + (seq.first + its) * a.out_token_stride + its_head * a.out_head_stride + c;
+        float* part = parts + ((int64_t)(seq.first + its) * a.q_heads + its_head) * D + c;
+        const float now = whole ? T::to_float(*out) : *part;
+        if (!(fabsf(now) < INFINITY)) sum += now;
+        if (whole) *out = (short)T::pack(sum, 0.0f);
+        else *part = sum;
     }
 }
 

@@ -1,0 +1,40 @@
+"""Attention at the ends of the types' ranges (leanstream_amd.decode.PagedAttention): values that are not finite where
+some tokens see them, values at fp16's largest, scores near fp32's lowest.
+"""
+import math
+
+import pytest
+
+from test_gpu_attention import Problem, log
+
+pytestmark = pytest.mark.gpu
+
+
+def place(p, s, key):
+    return int(p.table[s, key // p.page]), key % p.page
+
+
+@pytest.mark.parametrize("keys", [300, 2300])      # one piece, and split along the keys
+@pytest.mark.parametrize("dim,heads,kv_heads,n", [(128, 8, 2, 40), (64, 4, 4, 60), (256, 4, 2, 20), (128, 8, 2, 4)])
+@pytest.mark.parametrize("first,second,want", [(math.nan, math.inf, math.nan), (math.inf, -math.inf, math.nan),
+                                               (math.inf, math.inf, math.inf), (-math.inf, 1.0, -math.inf)])
+def test_what_is_not_finite_adds_up(torch_gpu, dim, heads, kv_heads, n, keys, first, second, want):
+    """One value among the keys that every token sees, one that only the last tokens see: a row's result is what
+    their sum is. The weights of both are large enough for the type (all scores are alike)."""
+    torch = torch_gpu
+    log("case:", dim, heads, n, keys, first, second)
+    p = Problem(torch, "float16", dim, heads, kv_heads, 16, [(n, keys)], spread=0.0)
+    late = keys - 2
+    for key, value in ((keys - n - 200, first), (late, second)):
+        at, slot = place(p, 0, key)
+        p.v[at, :, slot, 5] = value
+    p.on_gpu().enqueue()
+    torch.cuda.synchronize()
+    got = p.out.cpu().float()
+    both = list(range(n - 2, n))           # positions keys - 2 and keys - 1
+    before = list(range(n - 2))
+    sees_both, sees_one = got[both][:, :, 5], got[before][:, :, 5]
+    assert bool(sees_both.isnan().all()) if want != want else bool((sees_both == want).all())
+    assert bool(sees_one.isnan().all()) if first != first else bool((sees_one == first).all())
+    rest = [d for d in range(dim) if d != 5]
+    assert got[:, :, rest].isfinite().all()
