@@ -43,6 +43,11 @@ struct F16 {
         typedef _Float16 v2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, v2{(_Float16)a, (_Float16)b});
     }
+    // A mean of finite values is no larger than they are, but with weights that were rounded apart from their sum it may
+    // be by 2^-11, which past the largest fp16 would make an infinity of it.
+    static __device__ __forceinline__ float mean(float x) {
+        return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x;
+    }
     static __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0,
                                                       0, 0);
@@ -60,6 +65,7 @@ struct BF16 {
         typedef __bf16 v2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, v2{(__bf16)a, (__bf16)b});
     }
+    static __device__ __forceinline__ float mean(float x) { return x; }   // its range is fp32's, and so is the sums'
     static __device__ __forceinline__ f32x16 mfma32(s16x8 a, s16x8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c,
                                                        0, 0, 0);
@@ -386,7 +392,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
         const int64_t token = seq.first + r / group, q_head = head * group + r % group;
         const float inv = sum > 0.0f ? 1.0f / sum : sum;   // NaN stays NaN
         *(uint32_t*)((short*)a.out + token * a.out_token_stride + q_head * a.out_head_stride + c) =
-            T::pack(x * inv, y * inv);
+            T::pack(T::mean(x * inv), T::mean(y * inv));
         if (a.lse && c == 0) a.lse[token * a.q_heads + q_head] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
     };
     for (int i = threadIdx.x; i < items; i += 64 * kRowWaves) {
@@ -843,7 +849,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
                     *(u32x2*)(out + 32 * d + 2 * i) =
-                        u32x2{T::pack(o[d][i] * inv, o[d][i + 1] * inv), T::pack(o[d][i + 2] * inv, o[d][i + 3] * inv)};
+                        u32x2{T::pack(T::mean(o[d][i] * inv), T::mean(o[d][i + 1] * inv)),
+                              T::pack(T::mean(o[d][i + 2] * inv), T::mean(o[d][i + 3] * inv))};
             if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
         } else {
 #pragma unroll
@@ -927,7 +934,7 @@ __global__ __launch_bounds__(1024) void attention_join_kernel(const ls_hip_atten
         const float inv = l > 0.0f ? 1.0f / l : l;   // NaN stays NaN
         short* out = (short*)a.out + (int64_t)t * a.out_token_stride + q_head * a.out_head_stride + kLane * lane;
 #pragma unroll
-        for (int i = 0; i < kLane; ++i) out[i] = (short)T::pack(o[i] * inv, 0.0f);
+        for (int i = 0; i < kLane; ++i) out[i] = (short)T::pack(T::mean(o[i] * inv), 0.0f);
         if (a.lse && lane == 0) a.lse[at] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
     }
 }

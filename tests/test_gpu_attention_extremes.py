@@ -38,3 +38,23 @@ def test_what_is_not_finite_adds_up(torch_gpu, dim, heads, kv_heads, n, keys, fi
     assert bool(sees_one.isnan().all()) if first != first else bool((sees_one == first).all())
     rest = [d for d in range(dim) if d != 5]
     assert got[:, :, rest].isfinite().all()
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(128, 32, 8), (64, 8, 8), (256, 8, 1)])
+@pytest.mark.parametrize("lengths", [[(1, k) for k in range(4, 60, 5)], [(30, 60), (20, 33)], [(1, 5000)], [(40, 3000)]])
+def test_values_at_the_largest_fp16(torch_gpu, dim, heads, kv_heads, lengths):
+    """A mean of values is no larger than they are, however its weights were rounded. All keys but one are alike, so
+    that their weights round the same way."""
+    torch = torch_gpu
+    log("case:", dim, heads, lengths)
+    for seed in (1, 2, 3):
+        p = Problem(torch, "float16", dim, heads, kv_heads, 16, lengths, seed=seed)
+        g = torch.Generator().manual_seed(seed)
+        p.k[:] = torch.randn(dim, generator=g).half()
+        for s, (_, keys) in enumerate(lengths):
+            at, slot = place(p, s, 0)
+            p.k[at, :, slot] += (0.5 * torch.randn(p.k[at, :, slot].shape, generator=g)).half()
+        p.v[:] = 65504.0
+        p.v[..., ::2] = -65504.0
+        p.on_gpu().enqueue()
+        p.check()
