@@ -321,8 +321,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
                     if (!sees(key, pos, window, sinks)) s[j / 4][j % 4] = -INFINITY;
                 }
             }
+            {   // rounded once: fused with the subtraction below, the best score's distance to itself would not be 0
+#pragma clang fp contract(off)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j / 4][j % 4] *= scale);
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j / 4][j % 4] *= scale);
+            }
             top = max32(max16(top));
             const float keep = __builtin_amdgcn_exp2f(m - top);
             m = top;
@@ -499,6 +502,9 @@ struct Tile {
 // A row's running maximum moves only where one of its scores (times scale log2(e)) exceeds it by more than this: until
 // then P is at most 2^8 instead of 1, and the sums need no scaling.
 constexpr float kSlack = 8.0f;
+// A maximum below it is rounded by 2^-5 at most, which its weights and their sum share. That of one beyond it is not
+// small beside 1, and scores have to be rounded alike before it is subtracted from them.
+constexpr float kFar = 0x1p20f;
 
 struct TilePlan {
     uint32_t splits;       // of a tile, at most
@@ -756,6 +762,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
 
     f32x16 o[D / 32] = {};
     float m = kNoKey, l = 0.0f;
+    float offset = m, trigger = m;   // what is subtracted from scaled scores; a score above needs a look at m
     bool later = false;
     if (begin < end) {
         f32x16 s[kSub];
@@ -794,13 +801,28 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
                 top = largest(s);
             }
             top = max32(top) * scale;
-            if (__any(top > m + kSlack)) {
+            if (__any(top > trigger)) {
                 // by a row's own scores: with the others' its roundings would hang on keys that it does not see
                 const float next_m = top > m + kSlack ? top : m, keep = __builtin_amdgcn_exp2f(m - next_m);
                 m = next_m;
                 l *= keep;
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) o[d] *= keep;
+                const bool far = fabsf(m) > kFar && m != kNoKey;
+                offset = far ? 0.0f : m;
+                trigger = far ? -INFINITY : m + kSlack;
+                if (__any(far)) {
+                    // rounded like the maximum before it is subtracted: fused into one step the distance could be
+                    // anything
+#pragma clang fp contract(off)
+#pragma unroll
+                    for (int kt = 0; kt < kSub; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float scaled = s[kt][i] * scale;
+                            s[kt][i] = far ? (scaled - m) / scale : s[kt][i];
+                        }
+                }
             }
             // The next tile's scores (after the last one: of what the buffer held before, unused), and this one's P
             // beside them: rounded to the values' type for the matrix product, summed in fp32.
@@ -810,8 +832,8 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
                 constexpr int kPairs = kKeys / 4, kSteps = D / 16;
 #pragma unroll
                 for (int pair = step * kPairs / kSteps; pair < (step + 1) * kPairs / kSteps; ++pair) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[pair / 8][pair % 8 * 2], scale, -m));
-                    const float y = __builtin_amdgcn_exp2f(fmaf(s[pair / 8][pair % 8 * 2 + 1], scale, -m));
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[pair / 8][pair % 8 * 2], scale, -offset));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(s[pair / 8][pair % 8 * 2 + 1], scale, -offset));
                     l += x + y;
                     p[pair / 4][pair % 4] = T::pack(x, y);
                 }

@@ -58,3 +58,40 @@ def test_values_at_the_largest_fp16(torch_gpu, dim, heads, kv_heads, lengths):
         p.v[..., ::2] = -65504.0
         p.on_gpu().enqueue()
         p.check()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dim,heads,kv_heads,lengths", [
+    (128, 8, 2, [(1, 120), (3, 40)]), (128, 8, 2, [(40, 90)]), (64, 4, 4, [(60, 128)]), (256, 4, 2, [(20, 100), (1, 9)]),
+    (128, 8, 2, [(40, 900)])])
+def test_scores_beyond_whole_numbers(torch_gpu, dim, heads, kv_heads, lengths, sign, dtype):
+    """Scores of 1e10 and more, whose neighbours in fp32 lie further apart than exponentials reach. Every product is
+    exact in fp32, and scores differ by 2^-8 of their size: all weight lies on the best visible key, or evenly on those
+    that share its score."""
+    torch = torch_gpu
+    log("case:", dim, heads, lengths, sign, dtype)
+    p = Problem(torch, dtype, dim, heads, kv_heads, 16, lengths)
+    p.q[:] = 2.0 ** 15
+    p.k.zero_()
+    g = torch.Generator().manual_seed(6)
+    step = {}
+    for s, (n, keys) in enumerate(lengths):
+        step[s] = torch.randperm(keys, generator=g) % 128
+        for key in range(keys):
+            at, slot = place(p, s, key)
+            p.k[at, :, slot] = sign * 2.0 ** 14 * (1 + float(step[s][key]) / 128)
+    p.on_gpu().enqueue()
+    torch.cuda.synchronize()
+    got, lse = p.out.cpu().double(), p.lse.cpu().double()
+    for s, (n, keys) in enumerate(lengths):
+        for i in range(n):
+            t = p.starts[s] + i
+            seen = sign * step[s][: keys - n + i + 1]
+            best = (seen == seen.max()).nonzero()[:, 0]
+            v = torch.stack([p.v[place(p, s, int(b))[0], :, place(p, s, int(b))[1]] for b in best]).double()
+            v = v.repeat_interleave(heads // kv_heads, 1)
+            want, size = v.mean(0), v.abs().mean(0)
+            assert ((got[t] - want).abs() <= p.u * want.abs() + (p.u + 2.0 ** -12) * size).all(), (s, i)
+            z = sign * 2.0 ** 29 * dim * (1 + sign * float(seen.max()) / 128) * p.scale
+            assert ((lse[t] - z - math.log(len(best))).abs() <= 2.0 ** -12 + 2.0 ** -20 * abs(z)).all()
