@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cerrno>
+#include <cfloat>
 #include <cmath>
 #include "leanstream_hip.h"
 #include "wave_ops.h"
@@ -31,8 +32,9 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// Below every score that can occur and finite: a row's maximum before its first visible key.
-constexpr float kNoKey = -1e30f;
+// A row's maximum before its first visible key: no finite score lies below it, and being finite itself it can be
+// subtracted from a masked one (-inf).
+constexpr float kNoKey = -FLT_MAX;
 
 // Bit patterns of the two 16-bit types; arithmetic is in fp32 and in the matrix instructions.
 struct F16 {
@@ -733,7 +735,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
         return key0 + kKeys - 1 <= low && (window == 0 || key0 > high - window || key0 + kKeys <= sinks);
     };
     auto largest = [&](const f32x16 (&s)[kSub]) {
-        float top = kNoKey;
+        float top = kNoKey;   // scaled like the scores it does not exceed any of them
 #pragma unroll
         for (int kt = 0; kt < kSub; ++kt)
 #pragma unroll

@@ -95,3 +95,37 @@ def test_scores_beyond_whole_numbers(torch_gpu, dim, heads, kv_heads, lengths, s
             assert ((got[t] - want).abs() <= p.u * want.abs() + (p.u + 2.0 ** -12) * size).all(), (s, i)
             z = sign * 2.0 ** 29 * dim * (1 + sign * float(seen.max()) / 128) * p.scale
             assert ((lse[t] - z - math.log(len(best))).abs() <= 2.0 ** -12 + 2.0 ** -20 * abs(z)).all()
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads,lengths", [
+    (128, 8, 2, [(1, 300), (3, 40)]), (64, 4, 4, [(1, 2500)]), (128, 8, 2, [(40, 300)]), (64, 4, 1, [(30, 2500)]),
+    (256, 4, 2, [(20, 200), (1, 9)])])
+def test_scores_near_the_lowest(torch_gpu, dim, heads, kv_heads, lengths):
+    """bf16 reaches scores of -1e31 and below. One dimension of q and k is not zero, its products are exact in fp32 and
+    differ by 2^-8 of their size and more: all weight lies on the best visible key, whose value is the result. The
+    logarithm of the sum is its score: 2^-20 of its size, as elsewhere."""
+    torch = torch_gpu
+    log("case:", dim, heads, lengths)
+    p = Problem(torch, "bfloat16", dim, heads, kv_heads, 16, lengths)
+    p.q.zero_()
+    p.q[..., 0] = 2.0 ** 60
+    p.k.zero_()
+    g = torch.Generator().manual_seed(4)
+    size = {}
+    for s, (n, keys) in enumerate(lengths):
+        j = torch.randperm(keys, generator=g)
+        size[s] = (1 + (j % 128) / 128).double() * 2.0 ** (46 + j // 128).double()
+        for key in range(keys):
+            at, slot = place(p, s, key)
+            p.k[at, :, slot, 0] = -float(size[s][key])
+    p.on_gpu().enqueue()
+    torch.cuda.synchronize()
+    got, lse = p.out.cpu(), p.lse.cpu().double()
+    for s, (n, keys) in enumerate(lengths):
+        for i in range(n):
+            p_i, t = keys - n + i, p.starts[s] + i
+            best = int(size[s][: p_i + 1].argmin())
+            at, slot = place(p, s, best)
+            assert torch.equal(got[t], p.v[at, :, slot].repeat_interleave(heads // kv_heads, 0)), (s, i)
+            z = -float(size[s][best]) * 2.0 ** 60 * p.scale
+            assert ((lse[t] - z).abs() <= 2.0 ** -20 * abs(z)).all()
