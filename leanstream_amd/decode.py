@@ -65,17 +65,46 @@ class _Call:
         # the handle alone: torch.cuda.current_stream() makes an object of it first, 1.9 us of a 3.5 us call
         self._current = functools.partial(torch._C._cuda_getCurrentRawStream, self._device.index)
         need = int(getattr(lib, f"ls_hip_{name}_workspace")(self._arg)) if hasattr(block, "workspace") else 0
-        if need and workspace is None:
-            workspace = torch.zeros(need, dtype=torch.uint8, device=self._device)
+        self._streams = None    # those in order with a workspace of the call's own
+        if need and workspace is None and torch.cuda.is_current_stream_capturing():
+            if name == "attention":     # its zeros would be part of the graph, and missing outside
+                raise RuntimeError("attention needs a workspace: bind it before the capture, or hand one in")
+            workspace = torch.empty(need, dtype=torch.uint8, device=self._device)
+        elif need and workspace is None:
+            with torch.cuda.device(self._device):
+                workspace = torch.zeros(need, dtype=torch.uint8, device=self._device)
+                self._zeroed = torch.cuda.Event()
+                self._zeroed.record()
+            self._streams = {self._current()}
         if workspace is not None:
             block.workspace, block.workspace_bytes = workspace.data_ptr(), workspace.numel()
         self.workspace = workspace
 
     def enqueue(self, stream=None):
-        """Put the call on `stream` (a hipStream_t handle; default: torch's current stream)."""
-        rc = self._enqueue(self._arg, self._current() if stream is None else stream)
+        """Put the call on `stream` (a hipStream_t handle; default: torch's current stream). A stream handed in
+        outlives the call, unless the call's workspace was handed in too."""
+        if stream is None:
+            stream = self._current()
+        if self._streams is not None and stream not in self._streams:
+            self._join(getattr(stream, "value", stream) or 0)
+        rc = self._enqueue(self._arg, stream)
         if rc:
             raise RuntimeError(f"Native {self.name} failed: {rc}")
+
+    def _join(self, handle):
+        """The caller does not see that the call's own workspace is zeroed on the stream on which it was bound, nor when it
+        is freed: another stream waits for the one, and the other waits for that stream's work."""
+        import torch
+
+        stream = torch.cuda.ExternalStream(handle, self._device) if handle else torch.cuda.default_stream(self._device)
+        if self._zeroed.query():
+            self._streams.add(handle)
+        else:
+            with torch.cuda.stream(stream):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(f"{self.name}: wait for the stream on which it was bound before the capture")
+            stream.wait_event(self._zeroed)
+        self.workspace.record_stream(stream)
 
 
 class PagedCache:
