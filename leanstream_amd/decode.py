@@ -64,6 +64,7 @@ class _Call:
 
         # the handle alone: torch.cuda.current_stream() makes an object of it first, 1.9 us of a 3.5 us call
         self._current = functools.partial(torch._C._cuda_getCurrentRawStream, self._device.index)
+        self._current_device = torch._C._cuda_getDevice
         need = int(getattr(lib, f"ls_hip_{name}_workspace")(self._arg)) if hasattr(block, "workspace") else 0
         self._streams = None    # those in order with a workspace of the call's own
         if need and workspace is None and torch.cuda.is_current_stream_capturing():
@@ -87,7 +88,13 @@ class _Call:
             stream = self._current()
         if self._streams is not None and stream not in self._streams:
             self._join(getattr(stream, "value", stream) or 0)
-        rc = self._enqueue(self._arg, stream)
+        if self._current_device() == self._device.index:
+            rc = self._enqueue(self._arg, stream)
+        else:       # the default stream's handle is 0 on every device: a launch goes to the current one
+            import torch
+
+            with torch.cuda.device(self._device):
+                rc = self._enqueue(self._arg, stream)
         if rc:
             raise RuntimeError(f"Native {self.name} failed: {rc}")
 
