@@ -516,6 +516,8 @@ struct TilePlan {
     uint64_t bytes;
 };
 constexpr uint64_t kPartsAt = 256;
+// Floats of a part: it begins at a multiple of 16 bytes, as it is stored in such words.
+__host__ __device__ inline uint64_t part_floats(uint64_t rows, uint64_t dim) { return (rows * (dim + 2) + 3) / 4 * 4; }
 constexpr uint32_t kLeastChunk = 8;    // steps: a split's part of the sums costs as much as one
 
 // Steps of `unit` keys that rows of up to `span` neighbouring tokens of a sequence see, at most.
@@ -863,7 +865,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
     l = sum32(l);
     const int64_t at = (int64_t)(seq.first + token) * a.q_heads + q_head;
     const int64_t part_rows = (int64_t)a.tokens * a.q_heads;
-    float* parts = (float*)((char*)a.workspace + plan.offset + kPartsAt) + work.split * part_rows * (D + 2);
+    float* parts = (float*)((char*)a.workspace + plan.offset + kPartsAt) + work.split * part_floats(part_rows, D);
     if (wave_row + col < row_end) {
         if (whole) {
             const float inv = l > 0.0f ? 1.0f / l : l;   // NaN stays NaN
@@ -946,7 +948,7 @@ __global__ __launch_bounds__(1024) void attention_join_kernel(const ls_hip_atten
         lane_sums o = {};
         float m = kNoKey, l = 0.0f;
 #pragma unroll 8
-        for (int begin = 0; begin < steps.count; begin += chunk, parts += part_rows * (D + 2)) {
+        for (int begin = 0; begin < steps.count; begin += chunk, parts += part_floats(part_rows, D)) {
             const f32x2 ml = *(const f32x2*)(parts + part_rows * D + 2 * at);
             const lane_sums x = *(const lane_sums*)(parts + at * D + kLane * lane);
             const float next = fmaxf(m, ml[0]), old = __builtin_amdgcn_exp2f(m - next);
@@ -1025,7 +1027,7 @@ TilePlan plan_tiles(const ls_hip_attention& a, uint64_t offset) {
     const uint64_t steps = most_steps(a.max_context, C::kKeys, C::kRows / group + 2, a.window, a.sinks);
     p.splits = (uint32_t)std::max<uint64_t>(1, std::min(C::kFill / least, (steps + kLeastChunk - 1) / kLeastChunk));
     p.offset = (std::max(offset, kCounterBytes) + 255) / 256 * 256;   // a call of few rows may use the counters next
-    const uint64_t part = (uint64_t)a.tokens * a.q_heads * (a.head_dim + 2) * sizeof(float);
+    const uint64_t part = part_floats((uint64_t)a.tokens * a.q_heads, a.head_dim) * sizeof(float);
     if (p.splits > 1) p.bytes = p.offset + kPartsAt + p.splits * part;
     return p;
 }
