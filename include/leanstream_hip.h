@@ -289,9 +289,9 @@ enum { LS_TYPE_F16 = 0, LS_TYPE_BF16 = 1, LS_TYPE_F32 = 2 };
  * whose context is out of bounds counts as one with no keys, one whose q_start is out of bounds as one with
  * no tokens, whose rows of out stay as they are (both: status RANGE); a key in a page outside [0, pages)
  * counts as a key and value of zeros (status BAD_DESCRIPTOR).
- * scale > 0; head_dim 64, 128 or 256; page_size a power of two; F16 or BF16 throughout; every pointer 16-byte
- * aligned and strides multiples of 8. The workspace (ls_hip_attention_workspace bytes, zeroed once by the
- * caller, then left alone) may be shared by calls that follow one another on one stream. */
+ * scale > 0; head_dim 64, 128 or 256; page_size a power of two; F16 or BF16 throughout; q, out, the pages and the
+ * workspace 16-byte aligned, the others 4-byte, strides multiples of 8. The workspace (ls_hip_attention_workspace
+ * bytes, zeroed once by the caller, then left alone) may be shared by calls that follow one another on one stream. */
 typedef struct ls_hip_attention {
     const void* q;                /* [tokens][q_heads][head_dim] */
     void* out;                    /* [tokens][q_heads][head_dim] */
@@ -369,11 +369,14 @@ int ls_hip_block_norm_enqueue(const ls_hip_block_norm* norm, void* stream);
  * the tokens are ranked by (logit descending, id ascending); of them keep the first top_k (top_k <= 0: all), of
  * these those whose better-ranked ones weigh less than top_p of all of these, of these those with e_i >= min_p;
  * the best one always stays. The token is the lowest kept id whose weight with the kept ids below it exceeds
- * uniform * (kept weight). Exponentials are fp32; with a filter they are weighed in whole steps of 2^-32 (less
- * than half a step: never drawn) and top_p and uniform in steps of 2^-24, without one summed in 64-bit floats in
- * a fixed order: equal inputs give equal results. temperature <= 0 (or NaN): the best token. NaN logits count as
- * -inf; a row without a logit above -inf gives token -1 and logprob -inf. logprob (optional): the logarithm of
- * e_token over the kept weight.
+ * uniform * (kept weight). Exponentials are fp32. With top_k, and with min_p alone, they are weighed in whole steps of
+ * 2^-32 (less than half a step: never drawn), top_p and uniform in steps of 2^-24. Without a filter, and with top_p but
+ * no top_k, the row's weight is a sum of fp32 exponentials, 8 or 16 at a time in fp32 and from there in 64-bit floats,
+ * in an order that the numbers of rows and logits fix; the share at which top_p cuts and that at which the token is drawn
+ * are then within 2^-20 of the definition's. Equal calls give equal results; a row whose top_p or uniform lies that near
+ * to the edge between two tokens may get the one or the other in a call of another number of rows.
+ * temperature <= 0 (or NaN): the best token. NaN logits count as -inf; a row without a logit above -inf gives token -1
+ * and logprob -inf. logprob (optional): the logarithm of e_token over the kept weight.
  * temperature, top_k, top_p, min_p: per row, or NULL for 1, all, 1, 0. vocab <= 2^20.
  * The workspace (ls_hip_sample_workspace bytes, any contents) may be shared by calls of this kind that follow
  * one another on one stream, not with attention's. */

@@ -2,7 +2,8 @@
 //
 // e_i = exp((l_i - top) / T), w_i = e_i in whole steps of 2^-32. Ranked by (logit descending, id ascending) the
 // kept tokens are a prefix of the ranking: everything above a cut logit, and of the tokens equal to it the
-// first few by id. Weights of a set are summed as whole numbers, so no order of atomics changes a result.
+// first few by id. Weights of a set are summed as whole numbers, so no order of atomics changes a result; only the weight
+// of a whole row (no filter, or top-p without top-k) is a sum of floats, chunk by chunk in a fixed order.
 //
 // One pass over the logits, in two launches. A workgroup of the first takes a chunk of a row and leaves its best token,
 // the sum of its exponentials and, in order of id, its candidates: as many of its largest logits as the record holds.
