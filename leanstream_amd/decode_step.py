@@ -59,7 +59,7 @@ class Step:
 
     def __init__(self, decoder, tokens, max_new):
         d = self.decoder = decoder
-        self.tokens = tokens
+        self.tokens, self.max_new = tokens, max_new
 
         def buffer(*shape, dtype=torch.float16):
             return torch.empty(shape, dtype=dtype, device=DEV)
@@ -109,8 +109,12 @@ class Step:
 
     def run(self, ids, lengths, uniform, temperature=0.0, top_p=1.0):
         """ids: the sequences' new tokens one after another; lengths: (new tokens, context with them) of each.
-        Returns the drawn token of every sequence (int32, on the GPU)."""
+        Returns the drawn token of every sequence (int32, on the GPU); that of one without new tokens means nothing."""
         d = self.decoder
+        if len(lengths) != d.sequences or ids.numel() != self.tokens or sum(n for n, _ in lengths) != self.tokens:
+            raise ValueError(f"the step is bound to {self.tokens} tokens of {d.sequences} sequences")
+        if not all(0 <= n <= min(k, self.max_new) and k <= d.max_context for n, k in lengths):
+            raise ValueError(f"a sequence of this step has up to {self.max_new} new tokens and {d.max_context} with them")
         ends = np.cumsum([0] + [n for n, _ in lengths])
         self.q_start.copy_(torch.from_numpy(ends.astype(np.int32)))
         self.context.copy_(torch.tensor([k for _, k in lengths], dtype=torch.int32))
