@@ -968,9 +968,11 @@ __global__ __launch_bounds__(1024) void attention_join_kernel(const ls_hip_atten
 bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
 int check(const ls_hip_attention& a) {
-    if (!a.q || !a.out || !a.k_pages || !a.v_pages || !a.page_table || !a.q_start || !a.context) return EINVAL;
-    if (!a.sequences || !a.q_heads || !a.kv_heads || a.q_heads % a.kv_heads || !a.pages || !a.table_width)
+    // the pointers of empty tensors may be NULL
+    if (a.tokens && (!a.q || !a.out || !a.k_pages || !a.v_pages || !a.page_table || !a.q_start || !a.context ||
+                     !a.sequences || !a.pages || !a.table_width))
         return EINVAL;
+    if (!a.q_heads || !a.kv_heads || a.q_heads % a.kv_heads) return EINVAL;
     if (!a.page_size || (a.page_size & (a.page_size - 1)) || a.dtype > LS_TYPE_F32) return EINVAL;
     if (a.tokens > 0x7fffffffu || a.pages > 0x7fffffffu || a.window > 0x3fffffffu || a.sinks > 0x3fffffffu ||
         a.max_context > 0x3fffffffu || (uint64_t)a.table_width * a.page_size < a.max_context || a.max_new > a.tokens)

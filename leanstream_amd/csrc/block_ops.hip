@@ -273,7 +273,8 @@ __global__ __launch_bounds__(Threads) void append_kernel(const ls_hip_append a, 
 bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
 int check(const ls_hip_block_norm& a) {
-    if (!a.block || !a.residual || (!a.hidden && !a.normed) || (a.normed && !a.pre_weight)) return EINVAL;
+    // the pointers of empty tensors may be NULL
+    if (a.rows && (!a.block || !a.residual || (!a.hidden && !a.normed) || (a.normed && !a.pre_weight))) return EINVAL;
     if (!a.width || a.dtype > LS_TYPE_F32 || !(a.eps >= 0.0f && a.eps < INFINITY)) return EINVAL;
     if (!(std::fabs(a.residual_scale) < INFINITY) || !(std::fabs(a.weight_offset) < INFINITY)) return EINVAL;
     const uintptr_t element = a.dtype == LS_TYPE_F32 ? 4 : 2;
@@ -289,11 +290,12 @@ int check(const ls_hip_block_norm& a) {
 }
 
 int check(const ls_hip_append& a) {
-    if (!a.k || !a.v || !a.k_pages || !a.v_pages || !a.page_table || !a.q_start || !a.context) return EINVAL;
-    if ((a.q_heads && (!a.q || !a.q_out)) || (a.rot && (!a.cos || !a.sin || !a.positions))) return EINVAL;
-    if (!a.sequences || !a.kv_heads || !a.head_dim || a.head_dim % 2 || a.rot % 2 || a.rot > a.head_dim) return EINVAL;
-    if (!a.page_size || (a.page_size & (a.page_size - 1)) || !a.pages || !a.table_width || a.dtype > LS_TYPE_F32)
+    if (a.tokens && (!a.k || !a.v || !a.k_pages || !a.v_pages || !a.page_table || !a.q_start || !a.context ||
+                     !a.sequences || !a.pages || !a.table_width || (a.q_heads && (!a.q || !a.q_out)) ||
+                     (a.rot && (!a.cos || !a.sin || !a.positions))))
         return EINVAL;
+    if (!a.kv_heads || !a.head_dim || a.head_dim % 2 || a.rot % 2 || a.rot > a.head_dim) return EINVAL;
+    if (!a.page_size || (a.page_size & (a.page_size - 1)) || a.dtype > LS_TYPE_F32) return EINVAL;
     if (a.tokens > 0x7fffffffu || a.sequences > 0x7fffffffu || a.pages > 0x7fffffffu) return EINVAL;
     if (a.table_stride < 0 || (a.sequences > 1 && a.table_stride < (int64_t)a.table_width)) return EINVAL;
     for (const void* p : {a.q, a.k, a.v, (const void*)a.q_out, (const void*)a.k_pages, (const void*)a.v_pages})

@@ -902,7 +902,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(const ls_hip_sampl
 bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
 int check(const ls_hip_sample& a) {
-    if (!a.logits || !a.uniform || !a.tokens || !a.vocab || a.dtype > LS_TYPE_F32) return EINVAL;
+    if (a.rows && (!a.logits || !a.uniform || !a.tokens || !a.vocab)) return EINVAL;
+    if (a.dtype > LS_TYPE_F32) return EINVAL;
     if (!aligned(a.logits, a.dtype == LS_TYPE_F32 ? 4 : 2) || a.row_stride < 0) return EINVAL;
     for (const void* p : {(const void*)a.uniform, (const void*)a.temperature, (const void*)a.top_k,
                           (const void*)a.top_p, (const void*)a.min_p, (const void*)a.tokens, (const void*)a.logprob})
