@@ -46,6 +46,11 @@ def _dtype(tensor, name):
     return TYPES[str(tensor.dtype)]
 
 
+def _stride(tensor, dim):
+    """Elements from one index to the next; 0 where there is only one, whose stride may be anything."""
+    return tensor.stride(dim) if tensor.shape[dim] > 1 else 0
+
+
 class _Call:
     """One bound call: the argument block, the tensors it points into, and the entry point."""
 
@@ -165,10 +170,10 @@ class PagedAttention(_Call):
         block = _native.Attention(
             q=_ptr(q), out=_ptr(out), lse=_ptr(lse), k_pages=_ptr(cache.k), v_pages=_ptr(cache.v),
             page_table=_ptr(page_table), q_start=_ptr(q_start), context=_ptr(context), status=_ptr(status),
-            q_token_stride=q.stride(0), q_head_stride=q.stride(1), out_token_stride=out.stride(0),
-            out_head_stride=out.stride(1), k_page_stride=cache.k.stride(0), k_head_stride=cache.k.stride(1),
-            k_slot_stride=cache.k.stride(2), v_page_stride=cache.v.stride(0), v_head_stride=cache.v.stride(1),
-            v_slot_stride=cache.v.stride(2), table_stride=page_table.stride(0), tokens=q.shape[0],
+            q_token_stride=_stride(q, 0), q_head_stride=_stride(q, 1), out_token_stride=_stride(out, 0),
+            out_head_stride=_stride(out, 1), k_page_stride=_stride(cache.k, 0), k_head_stride=_stride(cache.k, 1),
+            k_slot_stride=_stride(cache.k, 2), v_page_stride=_stride(cache.v, 0), v_head_stride=_stride(cache.v, 1),
+            v_slot_stride=_stride(cache.v, 2), table_stride=_stride(page_table, 0), tokens=q.shape[0],
             sequences=page_table.shape[0], q_heads=q.shape[1], kv_heads=cache.kv_heads, head_dim=cache.head_dim,
             pages=cache.pages, page_size=cache.page_size, table_width=page_table.shape[1],
             max_new=min(int(max_new), q.shape[0]), max_context=int(max_context), window=int(window), sinks=int(sinks),
