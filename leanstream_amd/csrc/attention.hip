@@ -6,6 +6,11 @@
 //
 // The query heads of one KV head share its keys, so the rows of a tile are (token, head of the group)
 // pairs: row r of a sequence is token r / group, head r % group.
+//
+// P = e^(s - m) is rounded to the values' type, the only type that the matrix cores multiply with them: P in two parts
+// would keep 32 bits at the price of a second product. It costs up to u |v| (u = 2^-11 in fp16, 2^-8 in bf16), as much as
+// the output's own rounding: against 64 bits, relative, 2.9e-4 for 4096 tokens over 32768 keys in fp16 where fp32
+// weights give 2.1e-4, and 2.2e-4 and 2.1e-4 for a single token. What is summed is the unrounded P.
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cerrno>
@@ -331,7 +336,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
             top = max32(max16(top));
             const float keep = __builtin_amdgcn_exp2f(m - top);
             m = top;
-            // P is rounded to the values' type for the matrix product; the sum takes it in fp32
+            // P is rounded to the values' type; the sum takes it in fp32
             u32x4 p;
             float sum = 0.0f;
 #pragma unroll
@@ -472,12 +477,17 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
 // of one row only and the P that it computed is already the second product's operand: key slots are permuted alike in P
 // and V^T, which a sum over keys allows. V^T comes out of LDS by transposing reads.
 //
-// Bound by the matrix cores and the vector units, which are busy for 45 % of the time each (16 products of 32 cycles
+// Bound by the matrix cores and the vector units, which are busy for 43 and 41 % of the time (16 products of 32 cycles
 // and as long a stretch of exponentials, sums and roundings for 32 x 64 scores), at 2.0 to 2.1 GHz under this load: the
 // scores of the next tile are multiplied while those of this one go through the softmax. Tiles come from memory without
 // passing registers, two buffers each of K and V, one barrier a tile. 4096 tokens over 32768 keys, 32 / 8 heads of 128:
-// 2.15 ms in fp16 (960 TFLOP/s; a product of 8192 x 8192 matrices reaches 1180), 2.0 ms in bf16 (1040 of
+// 2.17 ms in fp16 (950 TFLOP/s; a product of 8192 x 8192 matrices reaches 1180), 2.06 ms in bf16 (1000 of
 // 1240). 64 rows a wave halve the LDS reads, but their 512 registers leave one wave a SIMD: 3.3 ms.
+//
+// A prompt from its start (4096 tokens over as many keys, 16 heads of 64: 81 us, 425 TFLOP/s) has all its tiles under way
+// at once, and those of early tokens see few keys: waves live for 60 % of the launch, the matrix cores are busy for 16 %
+// and the vector units for 32 %. Heads of 256 (2048 tokens over 8192 keys, 16 heads: 484 us, 500 TFLOP/s) leave one
+// wave a SIMD, so that nothing runs beside its waits: 20 % and 28 %.
 //
 // Where tiles are few, their keys are split; the parts go to the workspace in fp32 and are joined in order by
 // attention_join_kernel (128 tokens over 32768 keys, 32 / 8 heads of 128: 1019 us whole, 97 in
@@ -485,8 +495,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_rows_kernel(const ls
 template <int D>
 struct Tile {
     // D = 256 needs twice the registers a row; D = 64 has fewer products to a score, and two workgroups of 4 waves on a
-    // compute unit overlap better than one of 8 (4096 tokens over 4096 keys, 16 heads: 82 and 102 us; D = 128, 4096
-    // over 32768: 2.37 and 2.14 ms).
+    // compute unit overlap better than one of 8 (4096 tokens over 4096 keys, 16 heads: 81 and 102 us; D = 128, 4096
+    // over 32768: 2.37 and 2.17 ms).
     static constexpr int kWaves = D == 128 ? 8 : 4;
     static constexpr uint32_t kFill = D == 64 ? 512 : 256;    // workgroups that run at once
     static constexpr int kRows = 32 * kWaves;
@@ -560,7 +570,7 @@ struct TileWork {
         longest = wave_max(longest, 0u);
         chunk = max(longest, 1u);
         if (plan.splits == 1 || 2 * tiles > C::kFill) return;
-        // no more than 2^8 tiles of fewer than 2^24 steps
+        // Tiles times steps pass 32 bits only for contexts near 2^30, where the search below then begins lower.
         chunk = max((wave_sum(total) * a.kv_heads + C::kFill - 1) / C::kFill, kLeastChunk);
         chunk = max(chunk, (longest + plan.splits - 1) / plan.splits);
         for (;;) {   // twice the even share makes at most C::kFill / 2 + tiles
@@ -829,7 +839,7 @@ __global__ __launch_bounds__(64 * Tile<D>::kWaves, D == 64 ? 2 : 1) void attenti
                 }
             }
             // The next tile's scores (after the last one: of what the buffer held before, unused), and this one's P
-            // beside them: rounded to the values' type for the matrix product, summed in fp32.
+            // beside them: rounded to the values' type, summed in fp32.
             f32x16 next[kSub];
             u32x4 p[kKeys / 16];
             scores(next, t + 1, [&](int step) LS_INLINE {
@@ -1002,7 +1012,9 @@ int check(const ls_hip_attention& a) {
 // Splits of the sequences that take the row kernel. Long ones make kFill workgroups (131072 keys, 16 groups: 144 us;
 // with half or twice as many 150 and 154). Splits of few steps pay only up to a workgroup a compute unit (32 sequences
 // of 500 keys, 256 groups: whole 15 us, in four 20), and one workgroup joins them all: with s steps, about sqrt(2 s)
-// splits cost least (8000 keys: 21 splits 13 us, 63 splits 18). A split has a step for each of its waves.
+// splits cost least (8000 keys of 8 KV heads: 21 splits 13 us, 63 splits 18). That is set by the join, not by the card:
+// with few KV heads most of it stays idle (131072 keys of one sequence: one KV head, 94 splits, 40 us, 1.7 TB/s; two
+// 42 us, 3.2; eight 105 us, 5.1). A split has a step for each of its waves.
 SplitPlan plan_rows(const ls_hip_attention& a) {
     SplitPlan p{};
     p.rows = (uint32_t)std::min<uint64_t>((uint64_t)a.max_new * (a.q_heads / a.kv_heads), kRows);

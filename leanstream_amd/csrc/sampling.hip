@@ -21,7 +21,7 @@
 // 51 MB (a greedy pick, which needs none of the steps, 13), one row of 32768 7 + 9. A row whose nucleus is wide costs
 // most: 64 rows of 131072, each with settings of its own, 13 + 37 us. One launch, in which a row's last chunk went on
 // with the row, gave the chunks half the waves (its registers): 73 us for 64 rows with top-k, where the first form in
-// two took 28 (now 22).
+// two took 28 (now 22). For a few rows, whose chunks do not fill the card with either, it was not measured.
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cerrno>
