@@ -16,6 +16,7 @@
 #include <cerrno>
 #include <cfloat>
 #include <cmath>
+#include "kernel_launch.h"
 #include "leanstream_hip.h"
 #include "wave_ops.h"
 
@@ -1074,30 +1075,26 @@ Plan make_plan(const ls_hip_attention& a) {
 }
 
 template <class T, int D>
-void launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
+hipError_t launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
     const uint32_t shift = __builtin_ctz(a.page_size);
-    if (plan.by_rows) {
-        const dim3 grid(plan.rows.splits * a.kv_heads, a.sequences);
-        if (a.page_size >= 16)
-            attention_rows_kernel<T, D, true><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan.rows);
-        else attention_rows_kernel<T, D, false><<<grid, 64 * kRowWaves, 0, stream>>>(a, shift, plan.rows);
-    }
-    if (plan.by_tiles) {
-        typedef Tile<D> C;
-        const uint32_t grid = tile_grid<D>(a);
-        if (a.page_size >= 16)
-            attention_tile_kernel<T, D, true><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
-        else attention_tile_kernel<T, D, false><<<grid, 64 * C::kWaves, 0, stream>>>(a, shift, plan.tiles);
-        if (plan.tiles.splits > 1)
-            attention_join_kernel<T, D><<<dim3(a.tokens, (a.q_heads + 15) / 16), 1024, 0, stream>>>(a, plan.tiles);
-    }
+    const bool large = a.page_size >= 16;
+    hipError_t e = hipSuccess;
+    if (plan.by_rows)
+        e = launch_kernel(large ? attention_rows_kernel<T, D, true> : attention_rows_kernel<T, D, false>,
+                          dim3(plan.rows.splits * a.kv_heads, a.sequences), 64 * kRowWaves, stream, a, shift, plan.rows);
+    if (plan.by_tiles && e == hipSuccess)
+        e = launch_kernel(large ? attention_tile_kernel<T, D, true> : attention_tile_kernel<T, D, false>,
+                          dim3(tile_grid<D>(a)), 64 * Tile<D>::kWaves, stream, a, shift, plan.tiles);
+    if (plan.by_tiles && plan.tiles.splits > 1 && e == hipSuccess)
+        e = launch_kernel(attention_join_kernel<T, D>, dim3(a.tokens, (a.q_heads + 15) / 16), 1024, stream, a, plan.tiles);
+    return e;
 }
 
 template <class T>
-void launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
-    if (a.head_dim == 64) launch<T, 64>(a, plan, stream);
-    else if (a.head_dim == 128) launch<T, 128>(a, plan, stream);
-    else launch<T, 256>(a, plan, stream);
+hipError_t launch(const ls_hip_attention& a, const Plan& plan, hipStream_t stream) {
+    return a.head_dim == 64    ? launch<T, 64>(a, plan, stream)
+           : a.head_dim == 128 ? launch<T, 128>(a, plan, stream)
+                               : launch<T, 256>(a, plan, stream);
 }
 
 }  // namespace
@@ -1116,8 +1113,6 @@ extern "C" int ls_hip_attention_enqueue(const ls_hip_attention* a, void* stream)
     if (!a->tokens || !a->max_new) return 0;
     const Plan plan = make_plan(*a);
     if (plan.bytes && (!a->workspace || a->workspace_bytes < plan.bytes)) return ENOSPC;
-    if (a->dtype == LS_TYPE_F16) launch<F16>(*a, plan, static_cast<hipStream_t>(stream));
-    else launch<BF16>(*a, plan, static_cast<hipStream_t>(stream));
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? 0 : static_cast<int>(e);
+    const auto st = static_cast<hipStream_t>(stream);
+    return static_cast<int>(a->dtype == LS_TYPE_F16 ? launch<F16>(*a, plan, st) : launch<BF16>(*a, plan, st));
 }

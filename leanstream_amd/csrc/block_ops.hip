@@ -6,6 +6,7 @@
 #include <cerrno>
 #include <cmath>
 #include <type_traits>
+#include "kernel_launch.h"
 #include "leanstream_hip.h"
 #include "wave_ops.h"
 
@@ -144,14 +145,15 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(const ls_hip_block
 }
 
 template <class T>
-void launch_norm(const ls_hip_block_norm& a, hipStream_t st) {
+hipError_t launch_norm(const ls_hip_block_norm& a, hipStream_t st) {
     const uint32_t w = a.width, packed = (a.rows + kThreads / 64 - 1) / (kThreads / 64);
-    if (w <= 512) block_norm_kernel<T, 1, 1><<<packed, kThreads, 0, st>>>(a);
-    else if (w <= 1024) block_norm_kernel<T, 1, 2><<<packed, kThreads, 0, st>>>(a);
-    else if (w <= 2048) block_norm_kernel<T, 1, 4><<<packed, kThreads, 0, st>>>(a);
-    else if (w <= 4096) block_norm_kernel<T, 4, 2><<<a.rows, kThreads, 0, st>>>(a);
-    else if (w <= 8192) block_norm_kernel<T, 4, 4><<<a.rows, kThreads, 0, st>>>(a);
-    else block_norm_kernel<T, 4, 8><<<a.rows, kThreads, 0, st>>>(a);
+    const auto kernel = w <= 512    ? block_norm_kernel<T, 1, 1>
+                        : w <= 1024 ? block_norm_kernel<T, 1, 2>
+                        : w <= 2048 ? block_norm_kernel<T, 1, 4>
+                        : w <= 4096 ? block_norm_kernel<T, 4, 2>
+                        : w <= 8192 ? block_norm_kernel<T, 4, 4>
+                                    : block_norm_kernel<T, 4, 8>;
+    return launch_kernel(kernel, dim3(w <= 2048 ? packed : a.rows), kThreads, st, a);
 }
 
 // Lengths and page tables do not change while a kernel runs: uniform ones come over the scalar cache.
@@ -314,11 +316,6 @@ int check(const ls_hip_append& a) {
     return 0;
 }
 
-int finish() {
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? 0 : static_cast<int>(e);
-}
-
 }  // namespace
 }  // namespace lsamd
 
@@ -328,10 +325,9 @@ extern "C" int ls_hip_block_norm_enqueue(const ls_hip_block_norm* a, void* strea
     if (const int rc = check(*a)) return rc;
     if (!a->rows) return 0;
     const auto st = static_cast<hipStream_t>(stream);
-    if (a->dtype == LS_TYPE_F16) launch_norm<_Float16>(*a, st);
-    else if (a->dtype == LS_TYPE_BF16) launch_norm<__bf16>(*a, st);
-    else launch_norm<float>(*a, st);
-    return finish();
+    return static_cast<int>(a->dtype == LS_TYPE_F16    ? launch_norm<_Float16>(*a, st)
+                            : a->dtype == LS_TYPE_BF16 ? launch_norm<__bf16>(*a, st)
+                                                       : launch_norm<float>(*a, st));
 }
 
 extern "C" int ls_hip_append_enqueue(const ls_hip_append* a, void* stream) {
@@ -347,9 +343,8 @@ extern "C" int ls_hip_append_enqueue(const ls_hip_append* a, void* stream) {
         const auto kernel = a->dtype == LS_TYPE_F16
                                 ? wide ? append_kernel<_Float16, true, n> : append_kernel<_Float16, false, n>
                                 : wide ? append_kernel<__bf16, true, n> : append_kernel<__bf16, false, n>;
-        kernel<<<a->tokens, n, 0, st>>>(*a, shift);
+        return launch_kernel(kernel, dim3(a->tokens), n, st, *a, shift);
     };
-    if (a->tokens <= kAppendFew) launch(std::integral_constant<uint32_t, kAppendThreads>());
-    else launch(std::integral_constant<uint32_t, kAppendThreads / 2>());
-    return finish();
+    return static_cast<int>(a->tokens <= kAppendFew ? launch(std::integral_constant<uint32_t, kAppendThreads>())
+                                                    : launch(std::integral_constant<uint32_t, kAppendThreads / 2>()));
 }

@@ -25,6 +25,7 @@
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cerrno>
+#include "kernel_launch.h"
 #include "leanstream_hip.h"
 #include "wave_ops.h"
 
@@ -928,19 +929,16 @@ RowArgs plan_rows(const ls_hip_sample& a, int* vecs) {
 }
 
 template <class T>
-void launch(ls_hip_sample a, hipStream_t st) {
+hipError_t launch(ls_hip_sample a, hipStream_t st) {
     int vecs;
     const RowArgs p = plan_rows(a, &vecs);
     const uint32_t rows = a.rows;
     for (uint32_t r = 0; r < rows; r += kRowBlock) {
         const dim3 grid(p.chunks, std::min(rows - r, kRowBlock));
-        if (vecs == 1) {
-            sample_chunk_kernel<T, 1><<<grid, kThreads, 0, st>>>(a, p);
-            sample_row_kernel<T, 1><<<grid.y, kThreads, 0, st>>>(a, p);
-        } else {
-            sample_chunk_kernel<T, 2><<<grid, kThreads, 0, st>>>(a, p);
-            sample_row_kernel<T, 2><<<grid.y, kThreads, 0, st>>>(a, p);
-        }
+        hipError_t e = launch_kernel(vecs == 1 ? sample_chunk_kernel<T, 1> : sample_chunk_kernel<T, 2>, grid, kThreads, st, a, p);
+        if (e == hipSuccess)
+            e = launch_kernel(vecs == 1 ? sample_row_kernel<T, 1> : sample_row_kernel<T, 2>, dim3(grid.y), kThreads, st, a, p);
+        if (e != hipSuccess) return e;
         a.logits = (const T*)a.logits + (int64_t)kRowBlock * a.row_stride;
         a.uniform += kRowBlock;
         a.tokens += kRowBlock;
@@ -950,6 +948,7 @@ void launch(ls_hip_sample a, hipStream_t st) {
         if (a.min_p) a.min_p += kRowBlock;
         if (a.logprob) a.logprob += kRowBlock;
     }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -970,9 +969,7 @@ extern "C" int ls_hip_sample_enqueue(const ls_hip_sample* a, void* stream) {
     if (!a->rows) return 0;
     if (!a->workspace || a->workspace_bytes < ls_hip_sample_workspace(a)) return ENOSPC;
     const auto st = static_cast<hipStream_t>(stream);
-    if (a->dtype == LS_TYPE_F16) launch<_Float16>(*a, st);
-    else if (a->dtype == LS_TYPE_BF16) launch<__bf16>(*a, st);
-    else launch<float>(*a, st);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? 0 : static_cast<int>(e);
+    return static_cast<int>(a->dtype == LS_TYPE_F16    ? launch<_Float16>(*a, st)
+                            : a->dtype == LS_TYPE_BF16 ? launch<__bf16>(*a, st)
+                                                       : launch<float>(*a, st));
 }
